@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 r"""Builds libfa2_4d_mask.so (gfx950) in-tree with hipcc, and the native eager
-host path _fa2_host.so (csrc/fa_host.cpp) with g++ against torch.
+host path _fa2_host.so (csrc/fa_host.cpp, fa_cache_host.cpp) with g++ against torch.
 
 Usage: python fa2-with-4d-mask_amd/build_ext.py [--jobs N] [--verbose] [--host-sanitize]
 
@@ -43,12 +43,14 @@ HOST_SANITIZE = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize
                  "-Xarch_host", "-fno-sanitize-recover=undefined", "-Xarch_host", "-fno-omit-frame-pointer",
                  "-Xarch_host", "-g"]
 SOURCES = ["fa_fwd.hip", "fa_bwd.hip", "fa_bwd_kv.hip", "fa_bwd_dq.hip", "fa_wide.hip", "fa_rows.hip", "fa_mask.hip", "fa_noalloc.hip",
-           "fa_api.cpp"]
+           "fa_prefix.hip", "fa_keyw.hip", "fa_evict.hip", "fa_rotary.hip", "fa_api.cpp", "fa_cache_api.cpp"]
+HOST_SOURCES = ["fa_host.cpp", "fa_cache_host.cpp"]
 # Per-file extra flags.  fa_bwd_kv.hip keeps its dK/dV accumulators in AGPRs
 # through inline asm and wants every other MFMA result in VGPRs (read by
-# VALU); fa_wide.hip and fa_rows.hip (head dim 256) keep their MFMA operands in
-# AGPRs and every MFMA result in VGPRs.
-EXTRA_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("fa_bwd_kv.hip", "fa_wide.hip", "fa_rows.hip")}
+# VALU); fa_wide.hip, fa_rows.hip and fa_prefix.hip (head dim 256) keep their MFMA
+# operands in AGPRs and every MFMA result in VGPRs; fa_keyw.hip reads its results there.
+EXTRA_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+               for f in ("fa_bwd_kv.hip", "fa_wide.hip", "fa_rows.hip", "fa_prefix.hip", "fa_keyw.hip")}
 ARCH = "gfx950"
 
 
@@ -84,20 +86,29 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 
 def build_host(verbose: bool = False) -> Path:
-    """The native eager host path (csrc/fa_host.cpp): a Python module against
-    torch's C++ API, host code only."""
+    """The native eager host path (HOST_SOURCES): a Python module against torch's
+    C++ API, host code only."""
     import sysconfig
 
     import torch
 
     root = Path(torch.__file__).resolve().parent
     LIBDIR.mkdir(exist_ok=True)
+    BUILD.mkdir(exist_ok=True)
     tmp = HOST.with_suffix(".so.tmp")
     inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
            Path(hipcc()).resolve().parent.parent / "include", sysconfig.get_paths()["include"]]
-    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
-          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{HERE.parent / 'include'}",
-          *(f"-isystem{i}" for i in inc), str(CSRC / "fa_host.cpp"), "-o", str(tmp), f"-L{root / 'lib'}",
+
+    def obj(src: str) -> Path:
+        o = BUILD / (Path(src).stem + ".o")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{HERE.parent / 'include'}",
+              *(f"-isystem{i}" for i in inc), "-c", str(CSRC / src), "-o", str(o)], verbose)
+        return o
+
+    with ThreadPoolExecutor(len(HOST_SOURCES)) as ex:
+        objs = list(ex.map(obj, HOST_SOURCES))
+    _run(["g++", "-shared", *map(str, objs), "-o", str(tmp), f"-L{root / 'lib'}",
           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"], verbose)
     os.replace(tmp, HOST)
     return HOST

@@ -15,6 +15,7 @@
 
 #include "fa2_4d_mask.h"
 #include "fa_kernels.h"
+#include "fa_status.h"
 
 namespace fa {
 int fwd_block_rows(int D, bool causal, bool mask, bool score);
@@ -26,8 +27,10 @@ hipError_t launch_fill_i32(int32_t* p, int64_t n, int32_t v, hipStream_t s);
 }  // namespace fa
 
 namespace {
-
 thread_local char g_err[512] = "no error";
+}  // namespace
+
+namespace fa {
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -49,6 +52,55 @@ int check_operand(const char* name, const void* p, int64_t sb, int64_t st, int64
                 (long long)sb, (long long)st, (long long)sh);
   return FA_OK;
 }
+
+int launch_status(hipError_t e, const char* what) {
+  if (e != hipSuccess) return fail(FA_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+  return FA_OK;
+}
+
+// Key ranges of the 256-row forward: `base` blocks of up to `nt` key tiles each
+// (fewer in causal blocks), one workgroup per CU at a time.  When the blocks
+// alone leave CUs idle, the split with the least estimated time, in us as
+// measured (bf16, Hq 8-32, Tq 256-4096, Tk 1024-16384, mask or not): a workgroup
+// costs 8 plus, per tile, 1.7 (head dim 128) or 1.1 (64), with the two-part P of
+// a mask or score 2.7 or 1.9 -- a quarter less with few CUs busy (clocks) -- and
+// a split adds 6 plus the fp32 partials' way to memory and back.  Tq 512, Tk
+// 8192, Hq 32, D 128: 169 us in one range, 82 in four (102 in two, 101 in six);
+// Tq 1024, Tk 1024, Hq 16: 30 in one, 35-47 in two to eight.
+//
+// `shared`: the causal head-dim-64 blocks of 128 rows, three per CU, which overlap
+// little: a block alone takes 0.76 a tile, a CU's blocks together 0.63 a tile, and a
+// head's blocks walk half of nt tiles on average.  Measured / estimated, in one, two,
+// three, four ranges: T 4096, Hq 8 58 45 43 45 / 57 45 44 47; T 2048, Hq 16 32 34 33
+// 34 / 32 33 34 37; T 1000, Hq 32 19 26 28 31 / 20 26 29 32.
+int fwd_key_split(int64_t base, int64_t nt, int64_t rows, int D, bool prec, bool shared) {
+  if (base >= (shared ? 3 : 1) * kCus) return 1;
+  const double tile = D == 64 ? (prec ? 1.9 : 1.1) : (prec ? 2.7 : 1.7);
+  int best = 1;
+  double best_us = 0;
+  for (int ns = 1; ns <= 16 && ns <= nt; ++ns) {
+    const int64_t wgs = base * ns, rounds = (wgs + kCus - 1) / kCus, nt_r = (nt + ns - 1) / ns;
+    const double clk = 0.75 + 0.25 * std::min(1.0, (double)wgs / kCus);
+    double us = shared ? 8 + std::max(0.76 * nt_r, 0.63 * base * nt / 2 / kCus) : rounds * (8 + clk * tile * nt_r);
+    if (ns > 1) us += 6 + 1.5e-6 * rows * ns * D;
+    if (ns == 1 || us < best_us) {
+      best = ns;
+      best_us = ns == 1 ? 0.95 * us : us;   // split only for a clear gain
+    }
+  }
+  return best;
+}
+
+}  // namespace fa
+
+namespace {
+
+using fa::aligned16;
+using fa::check_operand;
+using fa::fail;
+using fa::fwd_key_split;
+using fa::kCus;
+using fa::launch_status;
 
 // Rows of every head below 2^31 - 2^16: 32-bit row indices with room to
 // round any count up to a whole tile.
@@ -105,20 +157,15 @@ int check_mask_ws(const uint8_t* mask, const void* ws) {
   return FA_OK;
 }
 
-int launch_status(hipError_t e, const char* what) {
-  if (e != hipSuccess) return fail(FA_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
-  return FA_OK;
-}
-
 // dS tiles (16-bit, every stored 32x32 block; causal: blocks on or below the
 // diagonal) handed from the dK/dV kernel to the dQ kernel.  The workspace
 // holds the planes of a slice of (batch, kv-head) units, as many as fit the
 // caller's limit (all of them when they fit), in as few slices of nearly
 // equal size as that allows: the backward then runs the two kernels once per
 // slice.  0 units: not even one unit fits.
-// With a mask or a score each tile is a pair: dS rounded, then its rounding
+// With a mask, a score or a dq_mode each tile is a pair: dS rounded, then its rounding
 // residual (the dQ kernel adds both products).
-int ds_tile_parts(const FaBwdParams* p) { return p->mask || p->score ? 2 : 1; }
+int ds_tile_parts(const FaBwdParams* p) { return p->mask || p->score || p->dq_mode ? 2 : 1; }
 // Default limit (ds_limit_bytes = 0): a constant, so the route, the slices and
 // the head-group split depend on the problem alone.  The headline shape (B1
 // T8192 Hq32 Hk8 D128) needs exactly 4 GiB non-causal and runs unsliced.
@@ -278,8 +325,6 @@ Route route_of(const FaBwdParams* p) {
 int64_t dq_groups(const FaBwdParams* p, int rows) {
   return ds_slice_units(p) * (p->heads_q / p->heads_k) * ((p->seqlen_q + rows - 1) / rows);
 }
-constexpr int64_t kCus = 256;
-
 // Atomic mode with the dS tiles: when the 256-row blocks alone give every CU
 // a workgroup, each workgroup owns its rows and writes dQ (split 1: no fp32
 // atomics, no zeroing, no conversion -- 20-70 % faster than adding partials);
@@ -307,13 +352,22 @@ bool dq_atomics(const FaBwdParams* p) {
   const Route r = route_of(p);
   return r == kDsAtomic && dq_split_of(p) > 1;
 }
+// dQ as fp32 sums in dq_accum: for those atomics, or beside another key set's
+bool dq_sums(const FaBwdParams* p) { return dq_atomics(p) || p->dq_mode != 0; }
+// (batch, head) strides of dq_accum
+int64_t dqa_sh(const FaBwdParams* p) {
+  return p->dq_accum_stride_h ? p->dq_accum_stride_h : (int64_t)p->seqlen_q * p->head_dim;
+}
+int64_t dqa_sb(const FaBwdParams* p) {
+  return p->dq_accum_stride_b ? p->dq_accum_stride_b : (int64_t)p->heads_q * p->seqlen_q * p->head_dim;
+}
 
 // query rows per workgroup of the dQ-from-dS kernel: 512 (8 waves sharing
 // each K tile) when dQ is written directly at head dim 128 without a mask or
 // a score (whose tile pairs double the staging) and that still gives every CU
 // a workgroup, else 256
 int dq_rows(const FaBwdParams* p) {
-  if (p->head_dim != 128 || p->mask || p->score || dq_atomics(p)) return fa::kDqDsRows;
+  if (p->head_dim != 128 || p->mask || p->score || dq_sums(p)) return fa::kDqDsRows;
   return dq_groups(p, fa::kDqDsRowsWide) >= kCus ? fa::kDqDsRowsWide : fa::kDqDsRows;
 }
 
@@ -346,38 +400,6 @@ int choose_split(const FaBwdParams* p) {
   return split;
 }
 
-// Key ranges of the 256-row forward: `base` blocks of up to `nt` key tiles each
-// (fewer in causal blocks), one workgroup per CU at a time.  When the blocks
-// alone leave CUs idle, the split with the least estimated time, in us as
-// measured (bf16, Hq 8-32, Tq 256-4096, Tk 1024-16384, mask or not): a workgroup
-// costs 8 plus, per tile, 1.7 (head dim 128) or 1.1 (64), with the two-part P of
-// a mask or score 2.7 or 1.9 -- a quarter less with few CUs busy (clocks) -- and
-// a split adds 6 plus the fp32 partials' way to memory and back.  Tq 512, Tk
-// 8192, Hq 32, D 128: 169 us in one range, 82 in four (102 in two, 101 in six);
-// Tq 1024, Tk 1024, Hq 16: 30 in one, 35-47 in two to eight.
-//
-// `shared`: the causal head-dim-64 blocks of 128 rows, three per CU, which overlap
-// little: a block alone takes 0.76 a tile, a CU's blocks together 0.63 a tile, and a
-// head's blocks walk half of nt tiles on average.  Measured / estimated, in one, two,
-// three, four ranges: T 4096, Hq 8 58 45 43 45 / 57 45 44 47; T 2048, Hq 16 32 34 33
-// 34 / 32 33 34 37; T 1000, Hq 32 19 26 28 31 / 20 26 29 32.
-int fwd_key_split(int64_t base, int64_t nt, int64_t rows, int D, bool prec, bool shared) {
-  if (base >= (shared ? 3 : 1) * kCus) return 1;
-  const double tile = D == 64 ? (prec ? 1.9 : 1.1) : (prec ? 2.7 : 1.7);
-  int best = 1;
-  double best_us = 0;
-  for (int ns = 1; ns <= 16 && ns <= nt; ++ns) {
-    const int64_t wgs = base * ns, rounds = (wgs + kCus - 1) / kCus, nt_r = (nt + ns - 1) / ns;
-    const double clk = 0.75 + 0.25 * std::min(1.0, (double)wgs / kCus);
-    double us = shared ? 8 + std::max(0.76 * nt_r, 0.63 * base * nt / 2 / kCus) : rounds * (8 + clk * tile * nt_r);
-    if (ns > 1) us += 6 + 1.5e-6 * rows * ns * D;
-    if (ns == 1 || us < best_us) {
-      best = ns;
-      best_us = ns == 1 ? 0.95 * us : us;   // split only for a clear gain
-    }
-  }
-  return best;
-}
 // ---- how the forward runs ----------------------------------------------------
 // Few query rows: the rows of a kv-head's group packed into blocks of 32
 // (fa_rows.hip), which read the mask bytes themselves.  Its work grows with the
@@ -612,8 +634,11 @@ static int check_bwd(const FaBwdParams* p, int split) {
   if (!p->lse) return fail(FA_ERR_NULL, "lse is NULL");
   if (!p->delta) return fail(FA_ERR_NULL, "delta is NULL");
   if (!p->dead_flags) return fail(FA_ERR_NULL, "dead_flags is NULL");
-  if (dq_atomics(p) && !p->dq_accum) return fail(FA_ERR_WORKSPACE, "atomic dQ needs dq_accum (plan.needs_dq_accum)");
-  if (dq_atomics(p) && !aligned16(p->dq_accum)) return fail(FA_ERR_STRIDE, "dq_accum must be 16-byte aligned");
+  if (p->dq_mode < 0 || p->dq_mode > 3) return fail(FA_ERR_SHAPE, "dq_mode %d must be a sum of FA_DQ_KEEP and FA_DQ_ADD", p->dq_mode);
+  if (p->dq_accum_stride_b < 0 || p->dq_accum_stride_h < 0 || p->dq_accum_stride_b % 4 || p->dq_accum_stride_h % 4)
+    return fail(FA_ERR_STRIDE, "dq_accum strides must be non-negative multiples of 4");
+  if (dq_sums(p) && !p->dq_accum) return fail(FA_ERR_WORKSPACE, "%s needs dq_accum (plan.needs_dq_accum)", p->dq_mode ? "dq_mode" : "atomic dQ");
+  if (dq_sums(p) && !aligned16(p->dq_accum)) return fail(FA_ERR_STRIDE, "dq_accum must be 16-byte aligned");
   const int G = p->heads_q / p->heads_k;
   if (split < 1 || G % split != 0) return fail(FA_ERR_SHAPE, "kv_split %d must divide the group size %d", split, G);
   if (split > 1 && (!p->dk_accum || !p->dv_accum))
@@ -645,8 +670,8 @@ int fa_bwd_plan(const FaBwdParams* p, FaBwdPlan* plan) {
   const int G = p->heads_q / p->heads_k;
   if (split < 1 || G % split != 0) return fail(FA_ERR_SHAPE, "kv_split %d must divide the group size %d", split, G);
   plan->kv_split = split;
-  plan->needs_dq_accum = dq_atomics(p) ? 1 : 0;
-  plan->dq_accum_elems = dq_atomics(p) ? (int64_t)p->batch * p->seqlen_q * p->heads_q * p->head_dim : 0;
+  plan->needs_dq_accum = dq_sums(p) ? 1 : 0;
+  plan->dq_accum_elems = dq_sums(p) ? (int64_t)p->batch * p->seqlen_q * p->heads_q * p->head_dim : 0;
   // one fp32 slab per head-group part, fully overwritten (nothing to zero)
   plan->dkv_accum_zeroed = 0;
   plan->dkv_accum_elems = split > 1 ? (int64_t)split * p->batch * p->seqlen_k * p->heads_k * p->head_dim : 0;
@@ -668,7 +693,8 @@ int fa_bwd_preprocess(const FaBwdParams* p) {
   a.o = p->o; a.dout = p->dout; a.lse = p->lse; a.dead = p->dead_flags;
   a.delta = p->delta;
   a.lse_b = lse_b_of(p);
-  a.dq_accum = dq_atomics(p) ? p->dq_accum : nullptr;
+  a.dq_accum = dq_sums(p) && !(p->dq_mode & FA_DQ_ADD) ? p->dq_accum : nullptr;   // (zeroed)
+  a.dqa_sb = dqa_sb(p); a.dqa_sh = dqa_sh(p);
   a.osb = p->o_stride_b; a.ost = p->o_stride_t; a.osh = p->o_stride_h;
   a.dsb = p->do_stride_b; a.dst = p->do_stride_t; a.dsh = p->do_stride_h;
   a.olo = p->o_lo;
@@ -717,7 +743,9 @@ static fa::BwdArgs bwd_args(const FaBwdParams* p, int split) {
   a.ng = a.G;
   a.ds_p0 = 0;
   a.split = split;
-  a.do_dq = dq_atomics(p) ? 1 : 0;
+  a.do_dq = dq_sums(p) ? 1 : 0;
+  a.fine = p->dq_mode != 0;
+  a.dqa_sb = dqa_sb(p); a.dqa_sh = dqa_sh(p);
   a.dq_split = dq_split_of(p);
   a.scale = p->scale;
   float sl2f;
@@ -769,7 +797,7 @@ int fa_bwd(const FaBwdParams* p) {
       q.acc_mode = 0;
       const int rows = std::min(p->seqlen_q, 32 * k.q32_hi) - 32 * k.q32_lo;
       // 512-row blocks (8 waves sharing each K tile) when they still give every CU one
-      const bool wide = p->head_dim == 128 && !p->score &&
+      const bool wide = p->head_dim == 128 && !p->score && !q.do_dq &&
                         (int64_t)p->batch * p->heads_q * (rows / fa::kDqDsRowsWide) >= kCus;
       q.dq_rows = wide ? fa::kDqDsRowsWide : fa::kDqDsRows;
       q.nqt = (rows + q.dq_rows - 1) / q.dq_rows;
@@ -839,11 +867,10 @@ int fa_bwd_finalize(const FaBwdParams* p) {
     }
   }
   fa::CvtJobs jobs{};
-  if (dq_atomics(p)) {
+  if (dq_sums(p) && !(p->dq_mode & FA_DQ_KEEP)) {
     // dq_accum is head-major [B, Hq, Tq, D]
-    const int64_t D = p->head_dim, Tq = p->seqlen_q, Hq = p->heads_q;
     fa::CvtArgs c{p->dq_accum, p->dq, p->dq_stride_b, p->dq_stride_t, p->dq_stride_h,
-                  p->batch, p->seqlen_q, p->heads_q, columns(p), 1, 0, Hq * Tq * D, D, Tq * D};
+                  p->batch, p->seqlen_q, p->heads_q, columns(p), 1, 0, dqa_sb(p), p->head_dim, dqa_sh(p)};
     jobs.job[jobs.n++] = c;
   }
   if (split > 1) {
@@ -885,6 +912,7 @@ int fa_bwd_noalloc(const FaBwdParams* p) {
   q.ds_tiles = nullptr;
   q.ds_limit_bytes = -1;   // no dS tiles: dQ is recomputed
   q.atomic_dq = 0;
+  q.dq_mode = 0;
   q.kv_split = 1;          // dK/dV written by the kernel, no fp32 slabs
   q.delta = (float*)(uintptr_t)256;
   q.dead_flags = (int32_t*)(uintptr_t)256;

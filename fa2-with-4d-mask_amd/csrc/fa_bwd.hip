@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void preprocess_kernel(const PreArgs a) {
   acc += __shfl_xor(acc, 2);
   if (q < a.Tq) {
     if (a.dq_accum) {
-      float* z = a.dq_accum + (((int64_t)b * a.Hq + h) * a.Tq + q) * D + part * (D / 4);
+      float* z = a.dq_accum + b * a.dqa_sb + h * a.dqa_sh + (int64_t)q * D + part * (D / 4);
 #pragma unroll
       for (int u = 0; u < D / 16; ++u) *(f32x4*)(z + 4 * u) = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -116,8 +116,9 @@ constexpr int kDqBN = 64;    // keys per tile
 // keep one wave per SIMD: 256 registers would spill about a hundred.
 // FULL: all D columns of the operands exist; otherwise Dv do (tested at run time,
 // the score instance took 6-10 % longer, the others 1-4 %: T 2048, Hq 16, Hk 4).
-template <typename T, int D, bool CAUSAL, bool MASK, bool SCORE, bool FULL>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((MASK || SCORE) ? 1 : 2, (MASK || SCORE) ? 1 : 2)))
+// ACC: dQ is added to fp32 sums, dS always in two parts (one of two key sets that share a softmax).
+template <typename T, int D, bool CAUSAL, bool MASK, bool SCORE, bool FULL, bool ACC = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((MASK || SCORE || ACC) ? 1 : 2, (MASK || SCORE || ACC) ? 1 : 2)))
 void dq_kernel(const BwdArgs a) {
   using V8 = typename Vec8<T>::type;
   static_assert(D <= 128, "head dim 256 recomputes dQ in fa_wide.hip");
@@ -131,7 +132,7 @@ void dq_kernel(const BwdArgs a) {
   constexpr int U = BN * CH / 256;
   constexpr int OS = D + 8;
   static_assert(4 * 32 * OS <= 2 * (KT + VT), "dQ staging fits");
-  constexpr bool PREC = MASK || SCORE;
+  constexpr bool PREC = MASK || SCORE || ACC;
   __shared__ __attribute__((aligned(16))) T smem[2 * (KT + VT)];
 
   const int nblk = a.B * a.Hq * a.nqt;
@@ -327,6 +328,10 @@ void dq_kernel(const BwdArgs a) {
     e_nx = e_nx2;
   }
 
+  if constexpr (ACC) {
+    if (q0w + l32 < Tq) add_row_f32(a.dq_accum + b * a.dqa_sb + h * a.dqa_sh + (int64_t)(q0w + l32) * D, hf, qacc, 1.f);
+    return;
+  }
   T* os = smem + wave * 32 * OS;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -376,20 +381,21 @@ __global__ __launch_bounds__(256) void convert_kernel(const CvtJobs jobs) {
   }
 }
 
-template <typename T, int D, bool CAUSAL, bool FULL>
+template <typename T, int D, bool CAUSAL, bool FULL, bool ACC>
 hipError_t launch_dq_f(const BwdArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * a.Hq * a.nqt)), block(256);
   const bool m = a.mask != nullptr, sc = a.score != nullptr;
-  if (m && sc) hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, true, true, FULL>), grid, block, 0, s, a);
-  else if (m) hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, true, false, FULL>), grid, block, 0, s, a);
-  else if (sc) hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, false, true, FULL>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, false, false, FULL>), grid, block, 0, s, a);
+  if (m && sc) hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, true, true, FULL, ACC>), grid, block, 0, s, a);
+  else if (m) hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, true, false, FULL, ACC>), grid, block, 0, s, a);
+  else if (sc) hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, false, true, FULL, ACC>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((dq_kernel<T, D, CAUSAL, false, false, FULL, ACC>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
 template <typename T, int D, bool CAUSAL>
 hipError_t launch_dq_t(const BwdArgs& a, hipStream_t s) {
-  return a.Dv == D ? launch_dq_f<T, D, CAUSAL, true>(a, s) : launch_dq_f<T, D, CAUSAL, false>(a, s);
+  if (a.do_dq) return launch_dq_f<T, D, CAUSAL, false, true>(a, s);
+  return a.Dv == D ? launch_dq_f<T, D, CAUSAL, true, false>(a, s) : launch_dq_f<T, D, CAUSAL, false, false>(a, s);
 }
 
 template <typename T, int D>

@@ -308,7 +308,7 @@ __global__ __launch_bounds__(NW * 64, 2) void dq_ds_kernel(const BwdArgs a) {
     if (nloc == 0) return;   // no key step: nothing to add
     // fp32 partial rows [32][D] per step, then 64 consecutive floats per atomic instruction
     float* stf = (float*)smem + wv * 32 * OSF;
-    float* dqa = a.dq_accum + ((int64_t)b * a.Hq + h) * Tq * D;
+    float* dqa = a.dq_accum + b * a.dqa_sb + h * a.dqa_sh;
 #pragma unroll
     for (int i = 0; i < kDqSteps; ++i) {
 #pragma unroll
@@ -386,10 +386,10 @@ hipError_t launch_p(const BwdArgs& a, hipStream_t s) {
 }
 
 // A mask (PREC with the prepared lists) always has PREC; a score without a
-// mask runs the unmasked kernel with PREC.
+// mask, or a.fine, runs the unmasked kernel with PREC.
 template <typename T, int D, bool CAUSAL, bool ATOMIC>
 hipError_t launch_a(const BwdArgs& a, hipStream_t s) {
-  if (a.mask || a.score) return launch_p<T, D, CAUSAL, ATOMIC, true>(a, s);
+  if (a.mask || a.score || a.fine) return launch_p<T, D, CAUSAL, ATOMIC, true>(a, s);
   return launch_p<T, D, CAUSAL, ATOMIC, false>(a, s);
 }
 

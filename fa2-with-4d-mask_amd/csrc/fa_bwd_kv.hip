@@ -46,7 +46,9 @@ constexpr int kNBuf = 4;                 // LDS buffers of step tiles
 
 // FULL: all D columns of the operands exist (a run-time test cost 0.3-0.6 % of the
 // causal launch at B2 T4096 Hq32 Hk8 D128: registers and the first loads' order).
-template <typename T, int D, bool CAUSAL, bool MASK, bool SCORE, bool FULL>
+// FINE (no mask or score): dS in two parts all the same, for one of two key sets that share a
+// softmax, whose dQ cancel.
+template <typename T, int D, bool CAUSAL, bool MASK, bool SCORE, bool FULL, bool FINE = false>
 __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_eu(1, 1))) void dkdv2_kernel(const BwdArgs a) {
   using V8 = typename Vec8<T>::type;
   constexpr int DS = D / 16, NB = D / 32, CH = D / 8, ROWB = 2 * D;
@@ -82,7 +84,8 @@ __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_e
   // about one in a thousand of those entries a step off.  Each dS tile is
   // followed by the tile of its residuals for the dQ kernel.
   constexpr bool PREC = MASK || SCORE;
-  constexpr int NPART = PREC ? 2 : 1;   // 2 KB tiles per stored 32x32 block
+  constexpr bool DS2 = PREC || FINE;
+  constexpr int NPART = DS2 ? 2 : 1;    // 2 KB tiles per stored 32x32 block
   __shared__ __attribute__((aligned(1024))) char smem[LOFF + NBUF * LBUF];
 
   // ---- which (batch, kv-head, split, key block) ------------------------------
@@ -519,7 +522,7 @@ __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_e
   for (int nb = 0; nb < NB; ++nb) { dkt[nb] = f32x16{}; dvt[nb] = f32x16{}; }
   f32x16 sacc[2], pacc[2];   // S / dP of steps j (parity) ; lane: [q = 8 (i/4) + 4 hf + i%4][key]
   V8 ppk[2][2], dspk[2][2];  // P / dS packed: [parity][c], k-slot (hf, t) <-> row 16 c + 4 hf + t%4 + 8 (t/4)
-  V8 ppl[PREC ? 2 : 1][2], dsl[PREC ? 2 : 1][2];   // their rounding residuals (PREC)
+  V8 ppl[PREC ? 2 : 1][2], dsl[DS2 ? 2 : 1][2];    // their rounding residuals (PREC, DS2)
   V8 ppl2[PREC ? 2 : 1][2];                        // P's second residual (PREC)
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
@@ -530,7 +533,11 @@ __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_e
 #pragma unroll
   for (int x = 0; x < (PREC ? 2 : 1); ++x)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) { ppl[x][c] = V8{}; dsl[x][c] = V8{}; ppl2[x][c] = V8{}; }
+    for (int c = 0; c < 2; ++c) { ppl[x][c] = V8{}; ppl2[x][c] = V8{}; }
+#pragma unroll
+  for (int x = 0; x < (DS2 ? 2 : 1); ++x)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) dsl[x][c] = V8{};
 
   // S/dP of step j+1 (tile in buffer BUF+1) and dV/dK of step j-1 (buffer
   // BUF-1) -- one interleaved MFMA stream, with the P/dS VALU work of step j
@@ -641,6 +648,13 @@ __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_e
         dspk[PJ][c] = pack8<T>(pacc[PJ][8 * c + 0], pacc[PJ][8 * c + 1], pacc[PJ][8 * c + 2], pacc[PJ][8 * c + 3],
                                pacc[PJ][8 * c + 4], pacc[PJ][8 * c + 5], pacc[PJ][8 * c + 6], pacc[PJ][8 * c + 7]);
         asm volatile("" : "+v"(ppk[PJ][c]), "+v"(dspk[PJ][c]));
+        if constexpr (FINE) {
+          float r[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) r[t] = pacc[PJ][8 * c + t] - (float)(T)pacc[PJ][8 * c + t];
+          dsl[PJ][c] = pack8<T>(r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]);
+          asm volatile("" : "+v"(dsl[PJ][c]));
+        }
       } else {
         // keep the element's work in its slot (its result is first used later)
         asm volatile("" : "+v"(sacc[PJ][i]), "+v"(pacc[PJ][i]));
@@ -660,7 +674,7 @@ __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_e
       else pacc[PN] = mfma32(as_vec8<T>(xs[t % AHEAD]), vf[t >> 1], (t >> 1) == 0 ? nd_next : pacc[PN]);
       // dS of step j-1 out to its tile (non-temporal: read once, by the dQ kernel)
       if (t < 2) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, dspk[PN][t]), ds_rs, ds_vo + 1024 * t, 0, 2);
-      if constexpr (PREC) {   // the residual tile follows the tile
+      if constexpr (DS2) {   // the residual tile follows the tile
         if (t >= 2 && t < 4)
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, dsl[PN][t - 2]), ds_rs,
                                                  ds_vo + 2048 + 1024 * (t - 2), 0, 2);
@@ -676,7 +690,7 @@ __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_e
           }
         } else {
           mfma_acc(dkt[nb], xt[t % AHEAD], dspk[PN][c]);
-          if constexpr (PREC) mfma_acc(dkt[nb], xt[t % AHEAD], dsl[PN][c]);
+          if constexpr (DS2) mfma_acc(dkt[nb], xt[t % AHEAD], dsl[PN][c]);
         }
       }
       if (t + AHEAD < NOP) { xs[t % AHEAD] = rd_sd(t + AHEAD); xt[t % AHEAD] = rd_tr(t + AHEAD); }
@@ -717,8 +731,8 @@ __global__ __launch_bounds__(kKvWaves * 64, 1) __attribute__((amdgpu_waves_per_e
           if constexpr (PREC) {
             ppl[PJ][c] = __builtin_bit_cast(V8, __builtin_bit_cast(u32x4, ppl[PJ][c]) & mk);
             ppl2[PJ][c] = __builtin_bit_cast(V8, __builtin_bit_cast(u32x4, ppl2[PJ][c]) & mk);
-            dsl[PJ][c] = __builtin_bit_cast(V8, __builtin_bit_cast(u32x4, dsl[PJ][c]) & mk);
           }
+          if constexpr (DS2) dsl[PJ][c] = __builtin_bit_cast(V8, __builtin_bit_cast(u32x4, dsl[PJ][c]) & mk);
         }
       }
     }
@@ -919,6 +933,11 @@ hipError_t launch_f(const BwdArgs& a, hipStream_t s) {
 
 template <typename T, int D, bool CAUSAL>
 hipError_t launch_t(const BwdArgs& a, hipStream_t s) {
+  if (a.fine && !a.mask && !a.score) {
+    hipLaunchKernelGGL((dkdv2_kernel<T, D, CAUSAL, false, false, false, true>), dim3((unsigned)(a.nbk * a.nkt * a.nsp)),
+                       dim3(kKvWaves * 64), 0, s, a);
+    return hipGetLastError();
+  }
   return a.Dv == D ? launch_f<T, D, CAUSAL, true>(a, s) : launch_f<T, D, CAUSAL, false>(a, s);
 }
 

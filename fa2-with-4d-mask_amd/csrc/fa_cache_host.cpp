@@ -1,0 +1,348 @@
+// Native host path of the cache operators: outputs and workspaces from torch's allocator,
+// parameter blocks, launches on torch's current stream.  The Python wrappers (cache.py) have
+// checked shapes and types; their custom ops run the same functions.
+#include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/record_function.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+
+#include <cstring>
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "fa_host.h"
+
+namespace fa_host {
+namespace {
+
+// Entry points of libfa2_4d_mask.so as the Python loader resolved them.
+struct CacheApi {
+  int (*prefix_plan)(const FaPrefixParams*, FaPrefixPlan*);
+  int (*prefix_fwd)(const FaPrefixParams*);
+  int (*mask_plan)(const FaMaskParams*, int64_t*);
+  int (*mask_prepare)(const FaMaskParams*);
+  int (*key_weights_plan)(const FaKeyWeightsParams*, int64_t*);
+  int (*key_weights)(const FaKeyWeightsParams*);
+  int (*evict)(const FaEvictParams*);
+  int (*rotary)(const FaRotaryParams*);
+  const char* (*last_error)();
+};
+CacheApi g_api{};
+
+void check(int status, const char* what) {
+  TORCH_CHECK(status == FA_OK, what, " failed with status ", status, ": ", g_api.last_error());
+}
+
+using MaybeTensor = std::optional<Tensor>;
+Tensor get(const MaybeTensor& x) { return x.value_or(Tensor()); }
+MaybeTensor get_opt(const Tensor& x) { return x.defined() ? MaybeTensor(x) : std::nullopt; }
+
+// Columns the kernels are given of operands of D: D itself where they take it in place
+// (multiples of 16), else padded with zeros to their own head dim.
+int64_t columns(int64_t D) { return D % 16 == 0 ? D : kernel_head_dim(D); }
+
+// x as the kernels can address it; copies only where that does not hold.
+Tensor addressable(const Tensor& x, bool bhsd, int64_t W) {
+  Tensor y = x.size(3) == W ? x : at::constant_pad_nd(x, {0, W - x.size(3)});
+  return in_place(y, operand(y, bhsd)) ? y : y.clone(at::MemoryFormat::Contiguous);
+}
+
+// [B, T, H, D] memory, viewed in the caller's layout.
+Tensor token_major(int64_t B, int64_t T, int64_t H, int64_t D, const at::TensorOptions& o, bool bhsd) {
+  const Tensor x = at::empty({B, T, H, D}, o);
+  return bhsd ? x.transpose(1, 2) : x;
+}
+// The first D columns of such a tensor, in memory of their own.
+Tensor first_columns(const Tensor& x, int64_t D, bool bhsd) {
+  if (x.size(3) == D) return x;
+  return bhsd ? x.narrow(3, 0, D).transpose(1, 2).contiguous().transpose(1, 2) : x.narrow(3, 0, D).contiguous();
+}
+
+// A mask or score as [B|1, Hq|1, Tq, Tk] of its type with a contiguous key axis.
+Tensor side(const Tensor& x, at::ScalarType t) {
+  if (!x.defined()) return x;
+  Tensor y = x.scalar_type() == t ? x : x.to(t);
+  return y.size(3) == 1 || y.stride(3) == 1 ? y : y.contiguous();
+}
+
+Tensor key_axis_contiguous(const Tensor& x) { return x.size(2) == 1 || x.stride(2) == 1 ? x : x.contiguous(); }
+int64_t axis_stride(const Tensor& x, int i) { return x.size(i) == 1 ? 0 : x.stride(i); }
+
+template <typename P> void set_sides(P& p, const Tensor& mask, const Tensor& score, const Tensor& lengths) {
+  if (mask.defined()) {
+    p.mask = (const uint8_t*)mask.const_data_ptr();
+    p.mask_stride_b = side_stride(mask, 0); p.mask_stride_h = side_stride(mask, 1); p.mask_stride_q = side_stride(mask, 2);
+  }
+  if (score.defined()) {
+    p.score = (const float*)score.const_data_ptr();
+    p.score_stride_b = side_stride(score, 0); p.score_stride_h = side_stride(score, 1); p.score_stride_q = side_stride(score, 2);
+  }
+  if (lengths.defined()) p.lengths = (const int32_t*)lengths.const_data_ptr();
+}
+
+// kw [B, Hk, Tk] plus the sums of many rows' probabilities, from their LSE [B, Hq, Tq].
+Tensor key_weights(const Tensor& q_, const Tensor& k_, const Tensor& lse_, const MaybeTensor& lengths_, const MaybeTensor& mask_,
+                   const MaybeTensor& score_, const MaybeTensor& kw_, double scale, bool causal, bool bhsd) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard on_device(q_.device());
+  const int64_t D = q_.size(3), W = columns(D);
+  const Tensor q = addressable(q_, bhsd, W), k = addressable(k_, bhsd, W), lse = lse_.contiguous();
+  const Operand oq = operand(q, bhsd), ok = operand(k, bhsd);
+  const Tensor mask = side(get(mask_), at::kBool), score = side(get(score_), at::kFloat), lengths = get(lengths_);
+  FaKeyWeightsParams p{};
+  set_sides(p, mask, score, lengths);
+  p.q = oq.p; p.k = ok.p; p.lse = lse.const_data_ptr<float>();
+  p.q_stride_b = oq.sb; p.q_stride_t = oq.st; p.q_stride_h = oq.sh;
+  p.k_stride_b = ok.sb; p.k_stride_t = ok.st; p.k_stride_h = ok.sh;
+  p.batch = (int32_t)oq.B; p.seqlen_q = (int32_t)oq.T; p.seqlen_k = (int32_t)ok.T;
+  p.heads_q = (int32_t)oq.H; p.heads_k = (int32_t)ok.H;
+  p.head_dim = kernel_head_dim(D);
+  p.head_dim_in = (int32_t)W;
+  p.scale = (float)scale;
+  p.is_causal = causal;
+  p.dtype = dtype_code(q);
+  p.stream = stream_of(q);
+  Tensor kw = get(kw_);
+  if (kw.defined()) {
+    kw = key_axis_contiguous(kw);
+    p.kw_in = kw.const_data_ptr<float>();
+    p.kw_stride_b = axis_stride(kw, 0); p.kw_stride_h = axis_stride(kw, 1);
+  }
+  const Tensor out = at::empty({ok.B, ok.H, ok.T}, q.options().dtype(at::kFloat));
+  p.kw_out = out.data_ptr<float>();
+  int64_t bytes = 0;
+  check(g_api.key_weights_plan(&p, &bytes), "fa_key_weights_plan");
+  Tensor ws;
+  if (bytes) {
+    ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = bytes;
+  }
+  check(g_api.key_weights(&p), "fa_key_weights");
+  return out;
+}
+
+// The own keys' mask with `lengths` as part of it, for kernels that take none: rows broadcast.
+Tensor with_lengths(const Tensor& mask, const Tensor& lengths, int64_t B, int64_t Tq, int64_t Tk) {
+  if (!lengths.defined()) return mask;
+  const Tensor keep = at::arange(Tk, lengths.options()).lt(lengths.view({B, 1, 1, 1})).expand({B, 1, Tq, Tk});
+  return mask.defined() ? mask.logical_and(keep) : keep;
+}
+
+// O (in the caller's layout), LSE [B, Hq, Tq], O's rounding residual (empty unless asked for), key
+// weights [B, Hk, Tk] (empty unless asked for).
+std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& pk_,
+                                                  const MaybeTensor& pv_, const MaybeTensor& lengths_, const MaybeTensor& mask_,
+                                                  const MaybeTensor& score_, const MaybeTensor& kw_, double scale, bool causal,
+                                                  bool weights, bool residual, bool bhsd) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard on_device(q_.device());
+  RECORD_FUNCTION("tilelang_fa2_4d_mask::prefix_fwd", c10::ArrayRef<const c10::IValue>());
+  const int t = bhsd ? 2 : 1, h = bhsd ? 1 : 2;
+  const int64_t B = q_.size(0), Tq = q_.size(t), Hq = q_.size(h), D = q_.size(3), Tk = k_.size(t), Hk = k_.size(h);
+  const int64_t Tp = pk_ ? pk_->size(t) : 0, W = columns(D);
+  FaPrefixParams p{};
+  p.batch = (int32_t)B; p.seqlen_q = (int32_t)Tq; p.seqlen_p = (int32_t)Tp; p.seqlen_k = (int32_t)Tk;
+  p.heads_q = (int32_t)Hq; p.heads_k = (int32_t)Hk;
+  p.head_dim = kernel_head_dim(D);
+  p.head_dim_in = (int32_t)W;
+  p.scale = (float)scale;
+  p.is_causal = causal;
+  p.dtype = dtype_code(q_);
+  p.stream = stream_of(q_);
+  Tensor mask = Tk ? side(get(mask_), at::kBool) : Tensor(), lengths = Tk ? get(lengths_) : Tensor();
+  const Tensor score = Tk ? side(get(score_), at::kFloat) : Tensor();
+  set_sides(p, mask, score, lengths);
+  const bool kw_too = weights && Tk > 0;
+  Tensor kw = get(kw_), kw_out = at::empty({weights ? B : 0, Hk, Tk}, q_.options().dtype(at::kFloat));
+  if (kw_too) p.kw_out = kw_out.data_ptr<float>();
+  FaPrefixPlan plan{};
+  check(g_api.prefix_plan(&p, &plan), "fa_prefix_plan");
+  if (p.kw_out && !plan.few_rows) {   // the weights in a pass of their own, behind
+    p.kw_out = nullptr;
+    check(g_api.prefix_plan(&p, &plan), "fa_prefix_plan");
+  }
+  if (!plan.few_rows && lengths.defined()) {
+    mask = with_lengths(mask, lengths, B, Tq, Tk);
+    p.lengths = nullptr;
+    set_sides(p, mask, score, Tensor());
+    check(g_api.prefix_plan(&p, &plan), "fa_prefix_plan");
+  }
+
+  const Tensor q = addressable(q_, bhsd, W), k = addressable(k_, bhsd, W), v = addressable(v_, bhsd, W);
+  const Operand oq = operand(q, bhsd), ok = operand(k, bhsd), ov = operand(v, bhsd);
+  p.q = oq.p; p.k = ok.p; p.v = ov.p;
+  p.q_stride_b = oq.sb; p.q_stride_t = oq.st; p.q_stride_h = oq.sh;
+  p.k_stride_b = ok.sb; p.k_stride_t = ok.st; p.k_stride_h = ok.sh;
+  p.v_stride_b = ov.sb; p.v_stride_t = ov.st; p.v_stride_h = ov.sh;
+  Tensor pk, pv;
+  if (Tp > 0) {
+    pk = addressable(*pk_, bhsd, W);
+    pv = addressable(*pv_, bhsd, W);
+    const Operand opk = operand(pk, bhsd), opv = operand(pv, bhsd);
+    p.pk = opk.p; p.pv = opv.p;
+    p.pk_stride_t = opk.st; p.pk_stride_h = opk.sh;
+    p.pv_stride_t = opv.st; p.pv_stride_h = opv.sh;
+  }
+  const Tensor out = token_major(B, Tq, Hq, W, q.options(), bhsd), lse = at::empty({B, Hq, Tq}, q.options().dtype(at::kFloat));
+  const Operand oo = operand(out, bhsd);
+  p.o = const_cast<void*>(oo.p);
+  p.o_stride_b = oo.sb; p.o_stride_t = oo.st; p.o_stride_h = oo.sh;
+  p.lse = lse.data_ptr<float>();
+  Tensor lo;
+  if (residual) {
+    lo = token_major(B, Tq, Hq, W, q.options(), bhsd);
+    const Operand ol = operand(lo, bhsd);
+    p.o_lo = const_cast<void*>(ol.p);
+    p.o_lo_stride_b = ol.sb; p.o_lo_stride_t = ol.st; p.o_lo_stride_h = ol.sh;
+  }
+  if (p.kw_out && kw.defined()) {
+    kw = key_axis_contiguous(kw);
+    p.kw_in = kw.const_data_ptr<float>();
+    p.kw_stride_b = axis_stride(kw, 0); p.kw_stride_h = axis_stride(kw, 1);
+  }
+  const auto bytes = q.options().dtype(at::kByte);
+  Tensor mask_ws;
+  if (plan.needs_mask_ws && mask.defined()) {
+    FaMaskParams m{};
+    m.mask = p.mask;
+    m.mask_stride_b = p.mask_stride_b; m.mask_stride_h = p.mask_stride_h; m.mask_stride_q = p.mask_stride_q;
+    m.batch = p.batch; m.seqlen_q = p.seqlen_q; m.seqlen_k = p.seqlen_k; m.heads_q = p.heads_q;
+    m.is_causal = p.is_causal;
+    m.stream = p.stream;
+    int64_t n = 0;
+    check(g_api.mask_plan(&m, &n), "fa_mask_plan");
+    mask_ws = at::empty({n}, bytes);
+    m.workspace = mask_ws.data_ptr();
+    check(g_api.mask_prepare(&m), "fa_mask_prepare");
+    p.mask_ws = m.workspace;
+  }
+  const Tensor ws = at::empty({plan.workspace_bytes}, bytes);
+  p.workspace = ws.data_ptr();
+  p.workspace_bytes = plan.workspace_bytes;
+  check(g_api.prefix_fwd(&p), "fa_prefix_fwd");
+  if (kw_too && !p.kw_out) kw_out = key_weights(q, k, lse, get_opt(lengths), mask_, get_opt(score), kw_, scale, causal, bhsd);
+  return {first_columns(out, D, bhsd), lse, residual ? first_columns(lo, D, bhsd) : at::empty({0}, q.options()), kw_out};
+}
+
+// K, V and weights of the kept keys, and their indices.
+std::tuple<Tensor, Tensor, Tensor, Tensor> evict(const Tensor& k_, const Tensor& v_, const Tensor& kw_, const MaybeTensor& lengths_,
+                                                 int64_t keep, int64_t recent, bool bhsd) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard on_device(k_.device());
+  RECORD_FUNCTION("tilelang_fa2_4d_mask::evict", c10::ArrayRef<const c10::IValue>());
+  auto rows = [](const Tensor& x) { return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous(); };
+  const Tensor k = rows(k_), v = rows(v_), kw = key_axis_contiguous(kw_), lengths = get(lengths_);
+  const Operand ok = operand(k, bhsd), ov = operand(v, bhsd);
+  std::vector<int64_t> shape = k.sizes().vec();
+  shape[bhsd ? 2 : 1] = keep;
+  const Tensor ko = at::empty(shape, k.options()), vo = at::empty(shape, k.options());
+  const Tensor kwo = at::empty({ok.B, ok.H, keep}, kw.options()), idx = at::empty({ok.B, ok.H, keep}, kw.options().dtype(at::kLong));
+  const Operand oo = operand(ko, bhsd);
+  FaEvictParams p{};
+  p.k = ok.p; p.v = ov.p; p.kw = kw.const_data_ptr<float>();
+  if (lengths.defined()) p.lengths = (const int32_t*)lengths.const_data_ptr();
+  p.k_out = ko.data_ptr(); p.v_out = vo.data_ptr(); p.kw_out = kwo.data_ptr<float>(); p.index_out = idx.data_ptr<int64_t>();
+  p.k_stride_b = ok.sb; p.k_stride_t = ok.st; p.k_stride_h = ok.sh;
+  p.v_stride_b = ov.sb; p.v_stride_t = ov.st; p.v_stride_h = ov.sh;
+  p.kw_stride_b = axis_stride(kw, 0); p.kw_stride_h = axis_stride(kw, 1);
+  p.out_stride_b = oo.sb; p.out_stride_t = oo.st; p.out_stride_h = oo.sh;
+  p.batch = (int32_t)ok.B; p.seqlen_k = (int32_t)ok.T; p.heads_k = (int32_t)ok.H; p.head_dim = (int32_t)ok.D;
+  p.keep = (int32_t)keep; p.recent = (int32_t)recent;
+  p.stream = stream_of(k);
+  check(g_api.evict(&p), "fa_evict");
+  return {ko, vo, kwo, idx};
+}
+
+using Pair = std::tuple<Tensor, Tensor>;
+
+Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Tensor& freq, const std::vector<int64_t>& sections,
+                bool adjacent, bool inverse, bool bhsd) {
+  const c10::DeviceGuard on_device(q_.device());
+  RECORD_FUNCTION("tilelang_fa2_4d_mask::rotary", c10::ArrayRef<const c10::IValue>());
+  auto rows = [](const Tensor& x) { return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous(); };
+  const Tensor q = rows(q_), k = rows(k_);
+  const Operand oq = operand(q, bhsd), ok = operand(k, bhsd);
+  const Tensor qo = token_major(oq.B, oq.T, oq.H, oq.D, q.options(), bhsd), ko = token_major(ok.B, ok.T, ok.H, ok.D, k.options(), bhsd);
+  if (q.numel() == 0) return {qo, ko};
+  const Operand wq = operand(qo, bhsd), wk = operand(ko, bhsd);
+  FaRotaryParams p{};
+  p.q = oq.p; p.k = ok.p; p.q_out = const_cast<void*>(wq.p); p.k_out = const_cast<void*>(wk.p);
+  p.positions = pos.const_data_ptr();
+  p.inv_freq = freq.const_data_ptr<float>();
+  p.q_stride_b = oq.sb; p.q_stride_t = oq.st; p.q_stride_h = oq.sh;
+  p.k_stride_b = ok.sb; p.k_stride_t = ok.st; p.k_stride_h = ok.sh;
+  p.qo_stride_b = wq.sb; p.qo_stride_t = wq.st; p.qo_stride_h = wq.sh;
+  p.ko_stride_b = wk.sb; p.ko_stride_t = wk.st; p.ko_stride_h = wk.sh;
+  p.pos_stride_a = axis_stride(pos, 0); p.pos_stride_b = axis_stride(pos, 1); p.pos_stride_t = axis_stride(pos, 2);
+  p.batch = (int32_t)oq.B; p.seqlen = (int32_t)oq.T; p.heads_q = (int32_t)oq.H; p.heads_k = (int32_t)ok.H;
+  p.head_dim = (int32_t)oq.D;
+  p.rotary = (int32_t)(2 * freq.numel());
+  p.axes = (int32_t)sections.size();
+  TORCH_CHECK(sections.size() <= FA_ROTARY_AXES, "at most ", (int)FA_ROTARY_AXES, " axes");
+  for (size_t i = 0; i < sections.size(); ++i) p.sections[i] = (int32_t)sections[i];
+  p.positions_64 = pos.scalar_type() == at::kLong;
+  p.adjacent = adjacent;
+  p.sign = inverse ? -1 : 1;
+  p.dtype = dtype_code(q);
+  p.stream = stream_of(q);
+  check(g_api.rotary(&p), "fa_rotary");
+  return {qo, ko};
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                const Tensor& pos, const Tensor& freq, std::vector<int64_t> sections,
+                                                bool adjacent, bool inverse, bool bhsd) {
+    ctx->save_for_backward({pos, freq});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["flags"] = (int64_t)(adjacent | inverse << 1 | bhsd << 2);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Pair r = rotary_run(q, k, pos, freq, sections, adjacent, inverse, bhsd);
+    return {std::get<0>(r), std::get<1>(r)};
+  }
+  // The rotation back of both gradients (one that does not reach the loss: zeros), itself
+  // differentiable.
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    auto r = Rotary::apply(g[0], g[1], s[0], s[1], ctx->saved_data["sections"].toIntVector(), (bool)(flags & 1),
+                           !(flags >> 1 & 1), (bool)(flags >> 2 & 1));
+    torch::autograd::variable_list out(8);
+    out[0] = r[0];
+    out[1] = r[1];
+    return out;
+  }
+};
+
+Pair rotary(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& freq, const std::vector<int64_t>& sections,
+            bool adjacent, bool inverse, bool bhsd) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad())) {
+    const auto r = Rotary::apply(q, k, pos, freq, sections, adjacent, inverse, bhsd);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rotary_run(q, k, pos, freq, sections, adjacent, inverse, bhsd);
+}
+
+void init_cache(const std::vector<uintptr_t>& fn) {
+  TORCH_CHECK(fn.size() == 9, "nine entry points expected");
+  g_api = CacheApi{(decltype(CacheApi::prefix_plan))fn[0],      (decltype(CacheApi::prefix_fwd))fn[1],
+                   (decltype(CacheApi::mask_plan))fn[2],        (decltype(CacheApi::mask_prepare))fn[3],
+                   (decltype(CacheApi::key_weights_plan))fn[4], (decltype(CacheApi::key_weights))fn[5],
+                   (decltype(CacheApi::evict))fn[6],            (decltype(CacheApi::rotary))fn[7],
+                   (decltype(CacheApi::last_error))fn[8]};
+}
+
+}  // namespace
+
+void bind_cache(pybind11::module_& m) {
+  using release = pybind11::call_guard<pybind11::gil_scoped_release>;
+  m.def("init_cache", &init_cache);
+  m.def("attend", &attend, release());
+  m.def("evict", &evict, release());
+  m.def("rotary", &rotary, release());
+}
+
+}  // namespace fa_host

@@ -222,6 +222,21 @@ __device__ __forceinline__ int tile_off(int r, int c) {
   return r * W + ((((c >> 3) ^ chunk_swz<W>(r))) << 3) + (c & 7);
 }
 
+// dQ of one row's columns (32 nb + 8 gi + 4 hf + 0..3 in entry 4 gi + t of acc[nb]) times scale,
+// added to the row's fp32 sums.  The caller's workgroup owns the row: plain adds.
+template <int NB> __device__ __forceinline__ void add_row_f32(float* row, int hf, const f32x16 (&acc)[NB], float scale) {
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int gi = 0; gi < 4; ++gi) {
+      f32x4* p = (f32x4*)(row + nb * 32 + gi * 8 + hf * 4);
+      f32x4 x = *p;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[t] += acc[nb][gi * 4 + t] * scale;
+      *p = x;
+    }
+}
+
 // A kernel's (only) argument, read again from memory: what only the epilogue
 // needs then does not occupy scalar registers through the main loop (the
 // compiler loads a by-value argument's fields once, at the start).

@@ -114,11 +114,13 @@ __device__ __forceinline__ void lds_barrier() {
 // FULL: all D columns of the operands exist; otherwise Dv do (a run-time value in the
 // prologue and the epilogue, 0.2-1.5 us of a launch: not where a short problem in one
 // range would notice).
-template <typename T, int D, bool CAUSAL, bool MASK, bool SCORE, bool SPLIT, bool FULL>
-__global__ __launch_bounds__(fwd_waves(D, CAUSAL, MASK, SCORE) * 64, fwd_waves(D, CAUSAL, MASK, SCORE) == 4 ? 3 : 1) void fwd_kernel(const FwdArgs a) {
+// FINE (a split without a mask or score): P enters O in two parts all the same, for a softmax
+// that goes on over another key set, whose backward takes Delta from an O that must match it.
+template <typename T, int D, bool CAUSAL, bool MASK, bool SCORE, bool SPLIT, bool FULL, bool FINE = false>
+__global__ __launch_bounds__(fwd_waves(D, CAUSAL, MASK || FINE, SCORE) * 64, fwd_waves(D, CAUSAL, MASK || FINE, SCORE) == 4 ? 3 : 1) void fwd_kernel(const FwdArgs a) {
   const int Dv = FULL ? D : a.Dv;
   using V8 = typename Vec8<T>::type;
-  constexpr int kWaves = fwd_waves(D, CAUSAL, MASK, SCORE), kThreads = kWaves * 64;
+  constexpr int kWaves = fwd_waves(D, CAUSAL, MASK || FINE, SCORE), kThreads = kWaves * 64;
   constexpr int BM = kWaves * 32, BN = kBN;
   constexpr int DS = D / 16;            // k-steps of S^T
   constexpr int NB = D / 32;            // 32-wide d blocks of O^T
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(fwd_waves(D, CAUSAL, MASK, SCORE) * 64, fwd_waves(D
   // rounded value and its rounding residual, one more MFMA each): rows that
   // see few keys (packed documents, steep position biases) would otherwise
   // carry the 16-bit rounding of their few large weights into O.
-  constexpr bool PREC = MASK || SCORE;
+  constexpr bool PREC = MASK || SCORE || FINE;
   constexpr int QOFF = 2 * NBUF * TILEB;                 // Q rows (QLDS): 32 per wave
   constexpr int QBYTES = QLDS ? kWaves * 32 * ROWB : 0;
   __shared__ __attribute__((aligned(1024))) char smem[2 * NBUF * TILEB + QBYTES];
@@ -878,7 +880,12 @@ hipError_t launch_fwd_t(const FwdArgs& a, hipStream_t s) {
 
 template <typename T, int D, bool CAUSAL>
 hipError_t launch_fwd_c(const FwdArgs& a, hipStream_t s) {
-  if (a.ns > 1) return launch_fwd_t<T, D, CAUSAL, true, false>(a, s);
+  if (a.fine && !a.mask && !a.score) {
+    const dim3 grid((unsigned)(a.B * a.Hq * a.nqt * a.ns)), block(fwd_waves(D, CAUSAL, true, false) * 64);
+    hipLaunchKernelGGL((fwd_kernel<T, D, CAUSAL, false, false, true, false, true>), grid, block, 0, s, a);
+    return hipGetLastError();
+  }
+  if (a.part_o) return launch_fwd_t<T, D, CAUSAL, true, false>(a, s);   // (also a single range's partial result)
   return a.Dv == D ? launch_fwd_t<T, D, CAUSAL, false, true>(a, s) : launch_fwd_t<T, D, CAUSAL, false, false>(a, s);
 }
 

@@ -119,6 +119,7 @@ struct FwdArgs {
   int ns;
   float* part_o;
   float* part_ml;
+  int fine;             // partial results without a mask or score: P in two parts all the same
 };
 
 struct PreArgs {
@@ -127,6 +128,7 @@ struct PreArgs {
   float* lse_b;         // LSE the backward kernels use [B, Hq, Tq]: the forward's, except
                         // -inf for a row whose kept keys all have -inf logits
   int32_t* dead; float* dq_accum;
+  int64_t dqa_sb, dqa_sh;
   int64_t osb, ost, osh, dsb, dst, dsh;
   const void* olo;      // optional: O's rounding residual (Delta = sum dO (O + olo))
   int64_t olsb, olst, olsh;
@@ -174,8 +176,10 @@ struct BwdArgs {
   int nqt;              // query tiles per (b, h) (dQ kernel)
   int dq_rows;          // query rows per dQ-from-dS workgroup: kDqDsRows or kDqDsRowsWide
   int split;            // query-head-group split of the dK/dV kernel
-  int do_dq;            // dQ accumulated with fp32 atomics into dq_accum (by the dQ-from-dS
-                        // kernel over dq_split key ranges)
+  int do_dq;            // dQ added to the fp32 sums dq_accum (by the dQ-from-dS kernel over
+                        // dq_split key ranges, with atomics; by the kernels that recompute it)
+  int64_t dqa_sb, dqa_sh;   // ... whose rows of a (batch, head) are contiguous
+  int fine;             // dS in two parts without a mask or score too (tile pairs)
   int dq_split;         // key ranges of the atomic dQ-from-dS kernel
   float scale;          // softmax scale (dS multiplier)
   float scale_log2;     // |scale| * log2(e)  (1 when zero_scale)

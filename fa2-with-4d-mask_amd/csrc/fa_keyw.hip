@@ -1,0 +1,293 @@
+// Key weights of many query rows on gfx950 (MI355X): for every own key the sum of its
+// probability over the rows of its kv-head's group,
+//   kw[b, kvh, j] += sum_{h in group, i} exp2(log2(e) scale (q_i k_j + score_ij) - lse_i),
+// from the LSE a forward left.  (Few rows: fa_prefix.hip, whose forward keeps its logits.)
+//
+//   key_weights_kernel   a workgroup of 4 waves per (256 keys (128 at head dim 256), part of
+//                        the row tiles, kv-head, sequence).  A wave keeps its 64 (32) keys as MFMA
+//                        operands in registers and walks the rows of the group 32 at a time: S^T
+//                        = K Q^T leaves 16 keys of one row per lane and fragment, which become
+//                        probabilities and are added in place; the sum over the lanes (rows)
+//                        comes once, at the end.  No LDS.  Sums are fp32.
+//   key_weights_sum_kernel  adds the parts, in order (deterministic), where few key blocks
+//                        leave CUs idle and the row tiles are cut into parts.
+//   far_rows_kernel      with a score: rows whose LSE is so large (masks of the type's lowest
+//                        value in all of the row) that it no longer holds the sum's logarithm get
+//                        their largest raw logit and their sum anew; others leave at once.
+#include "fa_cache.h"
+#include "fa_common.h"
+
+namespace fa {
+namespace {
+
+constexpr int kWaves = 4;
+template <int D> constexpr int frags() { return D == 256 ? 1 : 2; }   // 32-key fragments per wave
+
+__device__ __forceinline__ int own_length(const KeyWArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+}
+
+// The row lane l32 of a 32-row tile reads, of a kv-head's group: r = g Tq + tq.
+struct Row {
+  int g, tq;
+};
+__device__ __forceinline__ Row row_of(const KeyWArgs& a, int r) {
+  const int g = r / a.Tq;
+  return {g, r - g * a.Tq};
+}
+
+template <typename T, int DS> __device__ __forceinline__ void load_q(const KeyWArgs& a, u32x4 (&x)[DS], int b, int h, int tq, int hf) {
+  load_row(x, (const T*)a.q + b * a.qsb + h * a.qsh + (int64_t)tq * a.qst + hf * 8, a.Dv);
+}
+
+// K rows [k0, k0 + 32) as the MFMA's A operand; rows past n read zeros.
+template <typename T, int DS> __device__ __forceinline__ void load_keys(const KeyWArgs& a, const T* kp, int k0, int n, int l32, int hf,
+                                                                         typename Vec8<T>::type (&kf)[DS]) {
+  const int rows = min(n - k0, 32);
+  const bool ok = rows > 0;
+  const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (ok ? (int64_t)k0 * a.kst : 0)), (short)0,
+                                                    ok ? (int)((int64_t)(rows - 1) * a.kst * 2 + 2 * a.Dv) : 0, 0x00020000);
+  const uint32_t off = (uint32_t)(l32 * a.kst * 2) + (uint32_t)(hf * 16);
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds)
+    kf[ds] = as_vec8<T>((u32x4)__builtin_amdgcn_raw_buffer_load_b128(rs, off + 32 * ds, 16 * ds < a.Dv ? 0 : kNoRec, 0));
+}
+
+// Keep bits (bit 8 gi + e <-> key k0 + 8 gi + 4 hf + e) of a row whose first lim keys count.
+__device__ __forceinline__ uint32_t in_row(int lim, int k0, int hf) {
+  const int n = lim - (k0 + 4 * hf);
+  return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
+}
+__device__ __forceinline__ uint32_t mask_bits(const KeyWArgs& a, const uint8_t* mrow, int k0, int hf, int n) {
+  uint32_t w = 0;
+  const int k = k0 + 4 * hf;
+  if (a.mask4 && k0 + 32 <= n) {
+    uint32_t x[4];
+#pragma unroll
+    for (int gi = 0; gi < 4; ++gi) x[gi] = *(const uint32_t*)(mrow + k + 8 * gi);
+#pragma unroll
+    for (int gi = 0; gi < 4; ++gi)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w |= ((x[gi] >> (8 * e)) & 0xffu) != 0 ? 1u << (8 * gi + e) : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w |= mrow[min(k + 8 * (i >> 2) + (i & 3), n - 1)] != 0 ? 1u << (8 * (i >> 2) + (i & 3)) : 0u;
+  }
+  return w;
+}
+__device__ __forceinline__ f32x16 scores(const float* srow, int k0, int hf, int n, float sign) {
+  f32x16 x;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = sign * srow[min(k0 + 8 * (i >> 2) + 4 * hf + (i & 3), n - 1)];
+  return x;
+}
+
+template <typename T, int D, bool MASK, bool SCORE>
+__global__ __launch_bounds__(kWaves * 64, 2) void key_weights_kernel(const KeyWArgs a) {
+  using V8 = typename Vec8<T>::type;
+  constexpr int DS = D / 16, NF = frags<D>();
+  const int W = xcd_remap(blockIdx.x, a.B * a.Hk * a.ns * a.nkb);
+  const int kb = W % a.nkb, W1 = W / a.nkb;   // (causal: the first key blocks have the most rows)
+  const int sp = W1 % a.ns, bk = W1 / a.ns;
+  const int b = bk / a.Hk, kvh = bk - b * a.Hk;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = own_length(a, b);
+  const int k0 = (kb * kWaves + wave) * NF * 32;   // this wave's first key
+  const int R = a.G * a.Tq, nt = (R + 31) / 32;
+  const float c2 = a.scale_log2;
+  const uint32_t neg = a.qsign < 0.f ? 0x80008000u : 0u;
+
+  f32x16 acc[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) acc[f] = f32x16{};
+  if (k0 < n) {
+    const T* kp = (const T*)a.k + b * a.ksb + kvh * a.ksh;
+    V8 kf[NF][DS];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) load_keys<T, DS>(a, kp, k0 + 32 * f, n, l32, hf, kf[f]);
+    // the next tile some row of which sees key k0
+    auto next = [&](int t) __attribute__((always_inline)) -> int {
+      if (a.causal)
+        for (; t < nt; t += a.ns) {
+          const Row lo = row_of(a, t * 32), hi = row_of(a, min(t * 32 + 31, R - 1));
+          if (lo.g != hi.g || hi.tq >= k0) break;
+        }
+      return t;
+    };
+    u32x4 x[DS];
+    float e = 0.f;
+    auto load_tile = [&](int t) __attribute__((always_inline)) {
+      const int r = t * 32 + l32;
+      const Row q = row_of(a, min(r, R - 1));
+      load_q<T, DS>(a, x, b, kvh * a.G + q.g, q.tq, hf);
+      // rows past R: +inf, as a row without a kept key
+      e = r < R ? a.lse[((int64_t)b * a.Hq + kvh * a.G + q.g) * a.Tq + q.tq] : kPosInf;
+    };
+    int t = next(sp);
+    if (t < nt) load_tile(t);
+    while (t < nt) {
+      V8 qf[DS];
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec8<T>(only_cols(x[ds], ds, a.Dv, neg));
+      const Row q = row_of(a, min(t * 32 + l32, R - 1));
+      const int h = kvh * a.G + q.g;
+      float sub = 0.f, lse = e, mul = 1.f;
+      if constexpr (SCORE) {
+        if (far_max(lse) && lse != kPosInf) {
+          const float* ml = a.far_ml + 2 * (((int64_t)b * a.Hq + h) * a.Tq + q.tq);
+          sub = ml[0];
+          lse = 0.f;
+          mul = 1.0f / ml[1];
+        }
+      }
+      const int t_nx = next(t + a.ns);
+      if (t_nx < nt) load_tile(t_nx);
+      const int lim = a.causal ? min(n, q.tq + 1) : n;
+      const bool edge = MASK || a.zero_scale || a.causal || k0 + 32 * NF > n;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const int kk = k0 + 32 * f;
+        f32x16 s = f32x16{};
+        if constexpr (SCORE) s = scores(a.score + b * a.ssb + h * a.ssh + (int64_t)q.tq * a.ssq, kk, hf, n, a.qsign);
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) s = mfma32(kf[f][ds], qf[ds], s);
+        uint32_t w = ~0u;
+        if (edge) {
+          w = in_row(lim, kk, hf);
+          if constexpr (MASK) w &= mask_bits(a, a.mask + b * a.msb + h * a.msh + (int64_t)q.tq * a.msq, kk, hf, n);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            s[j] = (w >> (8 * (j >> 2) + (j & 3))) & 1u ? (a.zero_scale ? 0.f : s[j]) : kNegInf;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if constexpr (SCORE) acc[f][j] += exp2_fast(fmaf(s[j] - sub, c2, -lse)) * mul;
+          else acc[f][j] += exp2_fast(fmaf(s[j], c2, -lse));
+        }
+      }
+      t = t_nx;
+    }
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) acc[f][j] += __shfl_xor(acc[f][j], d);
+  }
+  // every lane of a half holds the sums of keys 8 (j / 4) + 4 hf + j % 4: lane l32 = j writes one
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    float v = acc[f][0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) v = l32 == j ? acc[f][j] : v;
+    const int j = k0 + 32 * f + 8 * (l32 >> 2) + 4 * hf + (l32 & 3);
+    if (l32 < 16 && j < a.Tk) {
+      if (a.ns > 1) a.part[((int64_t)sp * a.B * a.Hk + bk) * a.Tk + j] = v;
+      else a.kw_out[(int64_t)bk * a.Tk + j] = v + (a.kw_in ? a.kw_in[b * a.kwsb + kvh * a.kwsh + j] : 0.f);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void key_weights_sum_kernel(const KeyWArgs a) {
+  const int64_t n = (int64_t)a.B * a.Hk * a.Tk;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < n; x += (int64_t)gridDim.x * 256) {
+    const int j = (int)(x % a.Tk), bk = (int)(x / a.Tk);
+    float v = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < a.ns; ++i) v += a.part[i * n + x];
+    a.kw_out[x] = v + (a.kw_in ? a.kw_in[(bk / a.Hk) * a.kwsb + (bk % a.Hk) * a.kwsh + j] : 0.f);
+  }
+}
+
+// A wave per 32 rows of one head.
+template <typename T, int D, bool MASK>
+__global__ __launch_bounds__(64) void far_rows_kernel(const KeyWArgs a) {
+  using V8 = typename Vec8<T>::type;
+  constexpr int DS = D / 16;
+  const int nt = (a.Tq + 31) / 32;
+  const int t = blockIdx.x % nt, bh = blockIdx.x / nt;
+  const int b = bh / a.Hq, h = bh - b * a.Hq;
+  const int lane = threadIdx.x, l32 = lane & 31, hf = lane >> 5;
+  const int tq = min(t * 32 + l32, a.Tq - 1);
+  const int64_t ri = (int64_t)bh * a.Tq + tq;
+  const float lse = a.lse[ri];
+  if (!wave_any(far_max(lse) && lse != kPosInf)) return;
+  const int n = own_length(a, b), lim = a.causal ? min(n, tq + 1) : n;
+  const float c2 = a.scale_log2;
+  const T* kp = (const T*)a.k + b * a.ksb + (h / a.G) * a.ksh;
+  u32x4 x[DS];
+  V8 qf[DS], kf[DS];
+  load_q<T, DS>(a, x, b, h, tq, hf);
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec8<T>(only_cols(x[ds], ds, a.Dv, a.qsign < 0.f ? 0x80008000u : 0u));
+  float mr = kNegInf, l = 0.f;
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    load_keys<T, DS>(a, kp, k0, n, l32, hf, kf);
+    f32x16 s = scores(a.score + b * a.ssb + h * a.ssh + (int64_t)tq * a.ssq, k0, hf, n, a.qsign);
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) s = mfma32(kf[ds], qf[ds], s);
+    uint32_t w = in_row(lim, k0, hf);
+    if constexpr (MASK) w &= mask_bits(a, a.mask + b * a.msb + h * a.msh + (int64_t)tq * a.msq, k0, hf, n);
+    float mx = kNegInf;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      s[j] = (w >> (8 * (j >> 2) + (j & 3))) & 1u ? (a.zero_scale ? 0.f : s[j]) : kNegInf;
+      mx = fmaxf(mx, s[j]);
+    }
+    mx = fmaxf(mr, half_max(mx));
+    if (mx > mr) {
+      l = mr == kNegInf ? 0.f : l * exp2_fast((mr - mx) * c2);
+      mr = mx;
+    }
+    if (mr > kNegInf) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) l += exp2_fast((s[j] - mr) * c2);
+    }
+  }
+  l = half_sum(l);
+  if (hf == 0) {
+    a.far_ml[2 * ri] = mr;
+    a.far_ml[2 * ri + 1] = l;
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_t(const KeyWArgs& a, hipStream_t s) {
+  const bool m = a.mask != nullptr, sc = a.score != nullptr;
+  if (sc) {
+    const dim3 grid((unsigned)(a.B * a.Hq * ((a.Tq + 31) / 32)));
+    if (m) hipLaunchKernelGGL((far_rows_kernel<T, D, true>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((far_rows_kernel<T, D, false>), grid, dim3(64), 0, s, a);
+    if (const hipError_t e = hipGetLastError()) return e;
+  }
+  const dim3 grid((unsigned)(a.B * a.Hk * a.ns * a.nkb)), block(kWaves * 64);
+  if (m && sc) hipLaunchKernelGGL((key_weights_kernel<T, D, true, true>), grid, block, 0, s, a);
+  else if (m) hipLaunchKernelGGL((key_weights_kernel<T, D, true, false>), grid, block, 0, s, a);
+  else if (sc) hipLaunchKernelGGL((key_weights_kernel<T, D, false, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((key_weights_kernel<T, D, false, false>), grid, block, 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && a.ns > 1) {
+    const int64_t n = ((int64_t)a.B * a.Hk * a.Tk + 255) / 256;
+    hipLaunchKernelGGL(key_weights_sum_kernel, dim3((unsigned)min_i64(n, 1 << 16)), dim3(256), 0, s, a);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+template <typename T> hipError_t launch_d(const KeyWArgs& a, int D, hipStream_t s) {
+  if (D == 64) return launch_t<T, 64>(a, s);
+  if (D == 128) return launch_t<T, 128>(a, s);
+  if (D == 256) return launch_t<T, 256>(a, s);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+int keyw_block_keys(int D) { return kWaves * 32 * (D == 256 ? frags<256>() : frags<128>()); }
+
+hipError_t launch_key_weights(const KeyWArgs& a, int D, int dtype, hipStream_t s) {
+  return dtype == 0 ? launch_d<bf16>(a, D, s) : launch_d<f16>(a, D, s);
+}
+
+}  // namespace fa

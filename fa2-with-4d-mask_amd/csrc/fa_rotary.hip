@@ -1,0 +1,125 @@
+// Rotary positions of several axes on gfx950 (MI355X): column pair i of token (b, t) turns by
+// positions[axis(i), b, t] * freq[i], queries and keys in one launch.
+//
+// The angle: freq / 2 pi as a 64-bit binary fraction of a turn, times the position modulo
+// 2^64.  Whole turns fall off by themselves and the rest is good to 2^-32 of a turn at any
+// position (a product in fp32 has lost 0.06 rad at position 10^6).  Cosines and sines are made
+// once per token, into LDS, for all of its heads.
+//
+// What bounds it: reading and writing queries and keys once.
+#include "fa_cache.h"
+#include "fa_common.h"
+
+namespace fa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPairs = 128;   // head dims up to 256
+constexpr int kTok = 4;          // tokens of a workgroup
+
+// V columns per piece: 8 (16 bytes) or 1.
+template <typename T, int V, bool ADJ>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
+  __shared__ float cs[2][kTok][kMaxPairs];   // cosines, sines
+  const int64_t tok0 = (int64_t)blockIdx.x * kTok, ntok = (int64_t)a.B * a.T;
+  const int nt = (int)min_i64(kTok, ntok - tok0);
+  const int tid = threadIdx.x;
+  for (int x = tid; x < nt * a.R2; x += kThreads) {
+    const int tk = x / a.R2, i = x - tk * a.R2;
+    const int64_t bt = tok0 + tk;
+    const int64_t b = bt / a.T, t = bt - b * a.T;
+    int ax = 0;
+#pragma unroll
+    for (int e = 0; e < kRotaryAxes - 1; ++e) ax += e < a.naxes - 1 && i >= a.ends[e] ? 1 : 0;
+    const int64_t at = ax * a.psa + b * a.psb + t * a.pst;
+    const int64_t pos = a.pos64 ? ((const int64_t*)a.pos)[at] : ((const int32_t*)a.pos)[at];
+    const double turns = (double)a.freq[i] * 0.15915494309189533577;   // 1 / 2 pi
+    const double frac = turns - floor(turns);
+    const uint64_t turn = (uint64_t)(frac * 18446744073709551616.0);
+    const int32_t top = (int32_t)((turn * (uint64_t)pos) >> 32);       // in [-1/2, 1/2) turns, times 2^32
+    float s, c;
+    sincospif((float)top * 0x1p-31f, &s, &c);
+    if (!(fabs(turns) < 1e300)) s = c = __builtin_nanf("");
+    cs[0][tk][i] = c;
+    cs[1][tk][i] = s * a.sign;
+  }
+  __syncthreads();
+
+  // pieces of a head: NR turned (two at once without ADJ: columns c and c + R2), NC copied
+  const int NR = (ADJ ? 2 * a.R2 : a.R2) / V, NC = (a.D - 2 * a.R2) / V, NP = NR + NC;
+  const int H = a.Hq + a.Hk, step = kThreads / NP;
+  const int pc = tid % NP;
+  int h = tid / NP, tk = 0;
+  if (h >= step) return;
+  while (h >= H) {
+    h -= H;
+    ++tk;
+  }
+  typedef T TV __attribute__((ext_vector_type(V)));
+  while (tk < nt) {
+    const int64_t bt = tok0 + tk;
+    const int64_t b = bt / a.T, t = bt - b * a.T;
+    const bool isq = h < a.Hq;
+    const int hh = isq ? h : h - a.Hq;
+    const T* src = isq ? (const T*)a.q + b * a.qsb + t * a.qst + hh * a.qsh : (const T*)a.k + b * a.ksb + t * a.kst + hh * a.ksh;
+    T* dst = isq ? (T*)a.qo + b * a.qosb + t * a.qost + hh * a.qosh : (T*)a.ko + b * a.kosb + t * a.kost + hh * a.kosh;
+    if (pc >= NR) {
+      const int c = 2 * a.R2 + (pc - NR) * V;
+      *(TV*)(dst + c) = *(const TV*)(src + c);
+    } else if constexpr (ADJ) {
+      const int c = pc * V;
+      if constexpr (V == 1) {
+        const int i = c >> 1;
+        const float co = cs[0][tk][i], si = cs[1][tk][i];
+        const float x = (float)src[c], y = (float)src[c ^ 1];
+        dst[c] = (T)(c & 1 ? fmaf(x, co, y * si) : fmaf(x, co, -(y * si)));
+      } else {
+        const TV x = *(const TV*)(src + c);
+        TV y;
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          const float co = cs[0][tk][(c + e) >> 1], si = cs[1][tk][(c + e) >> 1];
+          const float u = (float)x[e], v = (float)x[e + 1];
+          y[e] = (T)fmaf(u, co, -(v * si));
+          y[e + 1] = (T)fmaf(v, co, u * si);
+        }
+        *(TV*)(dst + c) = y;
+      }
+    } else {
+      const int c = pc * V;
+      const TV x0 = *(const TV*)(src + c), x1 = *(const TV*)(src + a.R2 + c);
+      TV y0, y1;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float co = cs[0][tk][c + e], si = cs[1][tk][c + e];
+        const float u = (float)x0[e], v = (float)x1[e];
+        y0[e] = (T)fmaf(u, co, -(v * si));
+        y1[e] = (T)fmaf(v, co, u * si);
+      }
+      *(TV*)(dst + c) = y0;
+      *(TV*)(dst + a.R2 + c) = y1;
+    }
+    h += step;
+    while (h >= H) {
+      h -= H;
+      ++tk;
+    }
+  }
+}
+
+template <typename T> hipError_t launch_t(const RotaryArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)a.B * a.T + kTok - 1) / kTok)), block(kThreads);
+  if (a.vec && a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, 8, true>), grid, block, 0, s, a);
+  else if (a.vec) hipLaunchKernelGGL((rotary_kernel<T, 8, false>), grid, block, 0, s, a);
+  else if (a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, 1, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, block, 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s) {
+  return dtype == 0 ? launch_t<bf16>(a, s) : launch_t<f16>(a, s);
+}
+
+}  // namespace fa

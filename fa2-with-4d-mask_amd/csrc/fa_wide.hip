@@ -424,7 +424,8 @@ __global__ __launch_bounds__(256, 1) void fwd_wide_kernel(const FwdArgs a) {
 // ---------------------------------------------------------------------------
 // Without FULL the staging zeroes the missing columns (a select per staged
 // register, 2 % of the kernel).
-template <typename T, bool CAUSAL, bool MASK, bool SCORE, int WHICH, bool FULL>
+// FINE: P and dS in several parts without a mask or score too, as in fa_bwd_kv.hip.
+template <typename T, bool CAUSAL, bool MASK, bool SCORE, int WHICH, bool FULL, bool FINE = false>
 __global__ __launch_bounds__(256, 1) void kv_wide_kernel(const BwdArgs a) {
   using V8 = typename Vec8<T>::type;
   constexpr int D = kWD, DS = D / 16, NB = D / 32, CH = D / 8;
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(256, 1) void kv_wide_kernel(const BwdArgs a) {
   constexpr int U = 32 * CH / 256;      // 16-byte chunks per thread per tile and kind
   constexpr int OS = D + 8;
   static_assert(4 * 32 * OS <= 4 * QT, "epilogue staging fits in the tile buffers");
-  constexpr bool PREC = MASK || SCORE;
+  constexpr bool PREC = MASK || SCORE || FINE;
   __shared__ __attribute__((aligned(16))) T smem[4 * QT];          // [buf][Q | dO]
   __shared__ __attribute__((aligned(16))) float lsd[2][2][32];     // [buf][LSE | -Delta][row]
 
@@ -697,7 +698,8 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, uint32_t ld
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (FA_LDS void*)(uintptr_t)lds_addr, 16, voff, 0, 0, 0);
 }
 
-template <typename T, bool CAUSAL, bool MASK, bool SCORE, bool FULL>
+// (ACC: dQ is added to fp32 sums, as in fa_bwd.hip)
+template <typename T, bool CAUSAL, bool MASK, bool SCORE, bool FULL, bool ACC = false>
 __global__ __launch_bounds__(256, 1) void dq_wide_kernel(const BwdArgs a) {
   using V8 = typename Vec8<T>::type;
   constexpr int D = kWD, DS = D / 16, NB = D / 32, CH = D / 8;
@@ -711,7 +713,7 @@ __global__ __launch_bounds__(256, 1) void dq_wide_kernel(const BwdArgs a) {
   constexpr int KOFF = 0, VOFF = NKB * TILEB;
   constexpr int OS = D + 8;               // epilogue staging stride (elements)
   static_assert(4 * 32 * OS * 2 <= (NKB + NVB) * TILEB, "dQ staging fits in the tile buffers");
-  constexpr bool PREC = MASK || SCORE;
+  constexpr bool PREC = MASK || SCORE || ACC;
   __shared__ __attribute__((aligned(1024))) char smem[(NKB + NVB) * TILEB];
 
   // blocks as in the forward: causal longest first across all XCDs
@@ -967,6 +969,10 @@ __global__ __launch_bounds__(256, 1) void dq_wide_kernel(const BwdArgs a) {
 
   // ---- epilogue: dQ = scale acc, through wave-private LDS rows ----------------------
   const float scale = a.scale;
+  if constexpr (ACC) {
+    if (q0w + l32 < Tq) add_row_f32(a.dq_accum + b * a.dqa_sb + h * a.dqa_sh + (int64_t)(q0w + l32) * D, hf, acc, scale);
+    return;
+  }
   T* os = (T*)smem + wave * 32 * OS;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -991,14 +997,14 @@ __global__ __launch_bounds__(256, 1) void dq_wide_kernel(const BwdArgs a) {
   }
 }
 
-template <typename T, bool CAUSAL, bool FULL>
+template <typename T, bool CAUSAL, bool FULL, bool ACC>
 hipError_t launch_dq_w(const BwdArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * a.Hq * a.nqt)), block(256);
   const bool m = a.mask != nullptr, sc = a.score != nullptr;
-  if (m && sc) hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, true, true, FULL>), grid, block, 0, s, a);
-  else if (m) hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, true, false, FULL>), grid, block, 0, s, a);
-  else if (sc) hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, false, true, FULL>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, false, false, FULL>), grid, block, 0, s, a);
+  if (m && sc) hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, true, true, FULL, ACC>), grid, block, 0, s, a);
+  else if (m) hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, true, false, FULL, ACC>), grid, block, 0, s, a);
+  else if (sc) hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, false, true, FULL, ACC>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((dq_wide_kernel<T, CAUSAL, false, false, FULL, ACC>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
@@ -1017,7 +1023,8 @@ template <typename T, bool CAUSAL, int WHICH, bool FULL>
 hipError_t launch_kv_w(const BwdArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.nbk * a.nkt * a.split)), block(256);
   const bool m = a.mask != nullptr, sc = a.score != nullptr;
-  if (m && sc) hipLaunchKernelGGL((kv_wide_kernel<T, CAUSAL, true, true, WHICH, FULL>), grid, block, 0, s, a);
+  if (a.fine && !m && !sc) hipLaunchKernelGGL((kv_wide_kernel<T, CAUSAL, false, false, WHICH, false, true>), grid, block, 0, s, a);
+  else if (m && sc) hipLaunchKernelGGL((kv_wide_kernel<T, CAUSAL, true, true, WHICH, FULL>), grid, block, 0, s, a);
   else if (m) hipLaunchKernelGGL((kv_wide_kernel<T, CAUSAL, true, false, WHICH, FULL>), grid, block, 0, s, a);
   else if (sc) hipLaunchKernelGGL((kv_wide_kernel<T, CAUSAL, false, true, WHICH, FULL>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((kv_wide_kernel<T, CAUSAL, false, false, WHICH, FULL>), grid, block, 0, s, a);
@@ -1038,8 +1045,9 @@ hipError_t launch_fwd_c(const FwdArgs& a, bool causal, hipStream_t s) {
 
 template <typename T>
 hipError_t launch_dq_c(const BwdArgs& a, bool causal, hipStream_t s) {
-  if (a.Dv == kWD) return causal ? launch_dq_w<T, true, true>(a, s) : launch_dq_w<T, false, true>(a, s);
-  return causal ? launch_dq_w<T, true, false>(a, s) : launch_dq_w<T, false, false>(a, s);
+  if (a.do_dq) return causal ? launch_dq_w<T, true, false, true>(a, s) : launch_dq_w<T, false, false, true>(a, s);
+  if (a.Dv == kWD) return causal ? launch_dq_w<T, true, true, false>(a, s) : launch_dq_w<T, false, true, false>(a, s);
+  return causal ? launch_dq_w<T, true, false, false>(a, s) : launch_dq_w<T, false, false, false>(a, s);
 }
 
 template <typename T>

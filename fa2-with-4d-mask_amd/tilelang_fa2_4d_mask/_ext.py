@@ -26,10 +26,12 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 LIB_PATH = (Path(os.environ["FA2_4D_MASK_LIB"]) if os.environ.get("FA2_4D_MASK_LIB")
             else Path(__file__).resolve().parent / "_lib" / "libfa2_4d_mask.so")
 HOST_PATH = Path(__file__).resolve().parent / "_lib" / "_fa2_host.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 FA_DTYPE_BF16 = 0
 FA_DTYPE_FP16 = 1
+FA_DQ_KEEP = 1
+FA_DQ_ADD = 2
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -83,7 +85,8 @@ class FaBwdParams(ctypes.Structure):
         ("ds_limit_bytes", _i64),
         ("mask_ws o_lo", _vp),
         ("o_lo_stride_b o_lo_stride_t o_lo_stride_h ds_tiles_elems", _i64),
-        ("head_dim_in", _i32),
+        ("head_dim_in dq_mode", _i32),
+        ("dq_accum_stride_b dq_accum_stride_h", _i64),
     )
 
 
@@ -93,6 +96,64 @@ class FaMaskParams(ctypes.Structure):
         ("mask_stride_b mask_stride_h mask_stride_q", _i64),
         ("batch seqlen_q seqlen_k heads_q is_causal", _i32),
         ("workspace stream", _vp),
+    )
+
+
+class FaPrefixParams(ctypes.Structure):
+    _fields_ = _fields(
+        ("q pk pv k v o o_lo lse mask score lengths kw_in kw_out", _vp),
+        ("q_stride_b q_stride_t q_stride_h pk_stride_t pk_stride_h pv_stride_t pv_stride_h "
+         "k_stride_b k_stride_t k_stride_h v_stride_b v_stride_t v_stride_h o_stride_b o_stride_t o_stride_h "
+         "o_lo_stride_b o_lo_stride_t o_lo_stride_h mask_stride_b mask_stride_h mask_stride_q "
+         "score_stride_b score_stride_h score_stride_q kw_stride_b kw_stride_h", _i64),
+        ("batch seqlen_q seqlen_p seqlen_k heads_q heads_k head_dim head_dim_in", _i32),
+        ("scale", ctypes.c_float),
+        ("is_causal dtype", _i32),
+        ("stream workspace", _vp),
+        ("workspace_bytes", _i64),
+        ("mask_ws", _vp),
+    )
+
+
+class FaPrefixPlan(ctypes.Structure):
+    _fields_ = _fields(("few_rows prefix_split own_split needs_mask_ws", _i32), ("workspace_bytes", _i64))
+
+
+class FaKeyWeightsParams(ctypes.Structure):
+    _fields_ = _fields(
+        ("q k lse mask score lengths kw_in kw_out", _vp),
+        ("q_stride_b q_stride_t q_stride_h k_stride_b k_stride_t k_stride_h mask_stride_b mask_stride_h mask_stride_q "
+         "score_stride_b score_stride_h score_stride_q kw_stride_b kw_stride_h", _i64),
+        ("batch seqlen_q seqlen_k heads_q heads_k head_dim head_dim_in", _i32),
+        ("scale", ctypes.c_float),
+        ("is_causal dtype", _i32),
+        ("stream workspace", _vp),
+        ("workspace_bytes", _i64),
+    )
+
+
+class FaEvictParams(ctypes.Structure):
+    _fields_ = _fields(
+        ("k v kw lengths k_out v_out kw_out index_out", _vp),
+        ("k_stride_b k_stride_t k_stride_h v_stride_b v_stride_t v_stride_h kw_stride_b kw_stride_h "
+         "out_stride_b out_stride_t out_stride_h", _i64),
+        ("batch seqlen_k heads_k head_dim keep recent", _i32),
+        ("stream", _vp),
+    )
+
+
+ROTARY_AXES = 8
+
+
+class FaRotaryParams(ctypes.Structure):
+    _fields_ = _fields(
+        ("q k q_out k_out positions inv_freq", _vp),
+        ("q_stride_b q_stride_t q_stride_h k_stride_b k_stride_t k_stride_h qo_stride_b qo_stride_t qo_stride_h "
+         "ko_stride_b ko_stride_t ko_stride_h pos_stride_a pos_stride_b pos_stride_t", _i64),
+        ("batch seqlen heads_q heads_k head_dim rotary axes", _i32),
+        ("sections", _i32 * ROTARY_AXES),
+        ("positions_64 adjacent sign dtype", _i32),
+        ("stream", _vp),
     )
 
 
@@ -109,7 +170,8 @@ class FaBwdPlan(ctypes.Structure):
 
 
 EXPORTED = ("fa_fwd", "fa_fwd_plan", "fa_bwd_preprocess", "fa_bwd", "fa_bwd_finalize", "fa_bwd_plan", "fa_mask_plan",
-            "fa_mask_prepare", "fa_last_error", "fa_abi_version", "fa_bwd_noalloc")
+            "fa_mask_prepare", "fa_last_error", "fa_abi_version", "fa_bwd_noalloc", "fa_prefix_plan", "fa_prefix_fwd",
+            "fa_key_weights_plan", "fa_key_weights", "fa_evict", "fa_rotary")
 
 _lib = None
 _lock = threading.Lock()
@@ -148,6 +210,13 @@ def load_library(path: os.PathLike | None = None) -> ctypes.CDLL:
         lib.fa_mask_plan.restype = ctypes.c_int
         lib.fa_mask_prepare.argtypes = [ctypes.POINTER(FaMaskParams)]
         lib.fa_mask_prepare.restype = ctypes.c_int
+        for name, args in (
+            ("fa_prefix_plan", (FaPrefixParams, FaPrefixPlan)), ("fa_prefix_fwd", (FaPrefixParams,)),
+            ("fa_key_weights_plan", (FaKeyWeightsParams, ctypes.c_int64)),
+            ("fa_key_weights", (FaKeyWeightsParams,)), ("fa_evict", (FaEvictParams,)), ("fa_rotary", (FaRotaryParams,)),
+        ):
+            getattr(lib, name).argtypes = [ctypes.POINTER(t) for t in args]
+            getattr(lib, name).restype = ctypes.c_int
         lib.fa_last_error.argtypes = []
         lib.fa_last_error.restype = ctypes.c_char_p
         lib.fa_abi_version.argtypes = []
@@ -162,12 +231,17 @@ def load_library(path: os.PathLike | None = None) -> ctypes.CDLL:
 _host = None
 
 
-def load_host(general_backward, settings, ds_limit: int):
+def load_host(general_backward=None, settings=None, ds_limit: int = 0):
     """Loads (once) and returns the native eager host path (csrc/fa_host.cpp),
-    bound to the loaded library; raises RuntimeError if it is absent."""
+    bound to the loaded library; raises RuntimeError if it is absent.  The
+    arguments are those of its ``init`` (default: fa2.py's)."""
     global _host
     if _host is not None:
         return _host
+    if general_backward is None:
+        from . import fa2
+
+        general_backward, settings, ds_limit = fa2._general_backward, fa2, fa2.DS_LIMIT_DEFAULT
     lib = load_library()
     with _lock:
         if _host is not None:
@@ -181,7 +255,10 @@ def load_host(general_backward, settings, ds_limit: int):
             raise RuntimeError(f"{HOST_PATH}: ABI version {mod.ABI_VERSION} != {ABI_VERSION}, rebuild it")
         fns = (lib.fa_fwd_plan, lib.fa_fwd, lib.fa_mask_plan, lib.fa_mask_prepare, lib.fa_bwd_plan,
                lib.fa_bwd_preprocess, lib.fa_bwd, lib.fa_bwd_finalize)
+        cache = (lib.fa_prefix_plan, lib.fa_prefix_fwd, lib.fa_mask_plan, lib.fa_mask_prepare, lib.fa_key_weights_plan,
+                 lib.fa_key_weights, lib.fa_evict, lib.fa_rotary, lib.fa_last_error)
         mod.init([ctypes.cast(f, ctypes.c_void_p).value for f in fns], general_backward, settings, ds_limit)
+        mod.init_cache([ctypes.cast(f, ctypes.c_void_p).value for f in cache])
         _host = mod
         return mod
 

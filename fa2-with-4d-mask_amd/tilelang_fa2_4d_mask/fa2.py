@@ -297,13 +297,15 @@ def _forward_impl(q, k, v, Mask, Score, scale: float, is_causal: bool, residual:
 
 
 def _backward_impl(do, q, k, v, O, LSE, mask, score, mask_ws, mst, sst, scale: float, is_causal: bool,
-                   use_atomic_backward: bool, O_lo: Optional[torch.Tensor] = None):
+                   use_atomic_backward: bool, O_lo: Optional[torch.Tensor] = None, dq_sums=None):
     """Host side of the backward (python/fa2.py:490-556) on logical [B, T, H, D]
     operands (Q, K, V as given or as the forward's kernels saw them); returns
     dQ, dK, dV in the input dtype, [B, T, H, D] contiguous with D that of dO.
     ``O_lo``: the forward's rounding residual of O (with a mask or a score),
     added to O for Delta.  Head dims other than the kernels' run in place or
-    zero-padded (``_columns_in_place``)."""
+    zero-padded (``_columns_in_place``).  ``dq_sums``: (fp32 sums, dq_mode, batch
+    stride, head stride) where dQ is summed over several key sets; with
+    FA_DQ_KEEP the dQ returned is not written."""
     B, Tq, Hq, D_in = do.shape
     _, Tk, Hk, _ = k.shape
     D = kernel_head_dim(D_in)
@@ -336,6 +338,8 @@ def _backward_impl(do, q, k, v, O, LSE, mask, score, mask_ws, mst, sst, scale: f
     p.kv_split = 0
     p.dtype = _ext.dtype_code(q.dtype)
     p.ds_limit_bytes = ds_limit_bytes(dev)
+    if dq_sums is not None:
+        dq_acc, p.dq_mode, p.dq_accum_stride_b, p.dq_accum_stride_h = dq_sums
     # the plan depends on whether a mask / score is given (dS tile pairs)
     p.mask, p.score = _ext.ptr(mask), _ext.ptr(score)
     lib = _ext.load_library()
@@ -345,7 +349,8 @@ def _backward_impl(do, q, k, v, O, LSE, mask, score, mask_ws, mst, sst, scale: f
 
     delta = torch.empty((2, B, Hq, Tq), dtype=torch.float32, device=dev)   # Delta, backward LSE
     dead = torch.zeros((B * Hk,), dtype=torch.int32, device=dev)
-    dq_acc = torch.empty((B, Tq, Hq, D), dtype=torch.float32, device=dev) if plan.needs_dq_accum else None
+    if dq_sums is None:
+        dq_acc = torch.empty((B, Tq, Hq, D), dtype=torch.float32, device=dev) if plan.needs_dq_accum else None
     dk_acc = dv_acc = None
     if plan.dkv_accum_elems > 0:
         # one fully overwritten fp32 slab per head-group part, or the running

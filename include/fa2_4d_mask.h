@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define FA_ABI_VERSION 7
+#define FA_ABI_VERSION 8
 
 enum FaDtype { FA_DTYPE_BF16 = 0, FA_DTYPE_FP16 = 1 };
 
@@ -109,7 +109,7 @@ typedef struct FaBwdParams {
                                     row whose kept keys all have a -inf logit) */
   int32_t* dead_flags;           /* workspace [B * Hk] int32, zeroed by the caller */
   const uint8_t* mask; const float* score;
-  float* dq_accum;               /* workspace [B, Hq, Tq, D] fp32 contiguous, head-major (atomic dQ) */
+  float* dq_accum;               /* workspace [B, Hq, Tq, D] fp32 contiguous, head-major (atomic dQ, dq_mode) */
   float* dk_accum;               /* workspace of plan.dkv_accum_elems fp32, when that is > 0 (head-group
                                     split slabs, or the running sums over ranges of query rows) */
   float* dv_accum;               /* idem */
@@ -143,7 +143,17 @@ typedef struct FaBwdParams {
                                     whether a mask or a score is given), else FA_ERR_WORKSPACE */
   int32_t head_dim_in;           /* as in FaFwdParams, for every 16-bit operand and output (the fp32
                                     accumulators have all head_dim columns).  0: all head_dim */
+  int32_t dq_mode;               /* 0, or for key sets that share one softmax (lse, o those of the whole): a
+                                    call per set, their dQ summed in dq_accum in fp32.  FA_DQ_KEEP: dQ stays
+                                    in dq_accum (dq is not written); FA_DQ_ADD: dq_accum holds the sums so
+                                    far (it is not zeroed).  plan.needs_dq_accum is 1 with either, and dS
+                                    is carried in two parts as with a mask or a score: the sets' dQ cancel
+                                    where a row's weight lies on keys of both that point the same way */
+  int64_t dq_accum_stride_b, dq_accum_stride_h;  /* of dq_accum's (batch, head) blocks [Tq, D], multiples
+                                    of 4; 0: as contiguous */
 } FaBwdParams;
+
+enum FaDqMode { FA_DQ_KEEP = 1, FA_DQ_ADD = 2 };
 
 /* Mask preparation: the bool mask of a problem turned into the workspace the
  * attention kernels read (the mask as bits, row-major and transposed; the
@@ -165,7 +175,7 @@ typedef struct FaBwdPlan {
   int32_t kv_split;              /* >1: dK/dV of each head-group part go to fp32 dk_accum/dv_accum slabs,
                                     summed by fa_bwd_finalize */
   int32_t needs_dq_accum;        /* 1 if dq_accum is used: dQ added with fp32 atomics (atomic_dq = 1 and
-                                    dq_split > 1); else dQ is written directly */
+                                    dq_split > 1), or dq_mode; else dQ is written directly */
   int64_t dq_accum_elems;        /* B*Tq*Hq*D when used, else 0 */
   int64_t dkv_accum_elems;       /* kv_split > 1: B*Tk*Hk*D per slab (kv_split slabs); ranges of query
                                     rows (ds_elems) at kv_split 1: B*Tk*Hk*D, the running sums; written
@@ -263,6 +273,136 @@ int fa_bwd_noalloc(const FaBwdParams* p);
  * dtype, causality, atomic_dq, kv_split, ds_limit_bytes and whether mask / score
  * are non-NULL (with either, every dS block is stored as a pair of tiles). */
 int fa_bwd_plan(const FaBwdParams* p, FaBwdPlan* plan);
+
+/* ---- a cache's operators: shared prefixes, key weights, eviction, rotary positions -------
+ * No counterpart in the reference.  The conventions above hold: caller-owned buffers,
+ * strides in elements, validation before any launch, nothing kept between calls. */
+
+/* Attention over a prefix that all sequences share and each sequence's own keys:
+ *   O = softmax([Q Kp^T, Q K^T + Score] scale, own keys masked) [Vp; V],  plus LSE,
+ * and optionally the own keys' weights, kw_out[b, kvh, j] = kw_in[b, kvh, j] + the sum of
+ * key j's probability over the rows of the kv-head's group (rows without a kept key add
+ * nothing).  seqlen_p or seqlen_k may be 0 (not both). */
+typedef struct FaPrefixParams {
+  const void* q;                 /* [B, Tq, Hq, D] */
+  const void* pk; const void* pv;/* [Tp, Hk, D]; ignored with seqlen_p 0 */
+  const void* k; const void* v;  /* [B, Tk, Hk, D]; ignored with seqlen_k 0 */
+  void* o;                       /* [B, Tq, Hq, D] output */
+  void* o_lo;                    /* optional output like o: O's rounding residual */
+  float* lse;                    /* [B, Hq, Tq] fp32 output, contiguous, as fa_fwd's */
+  const uint8_t* mask;           /* optional, over the own keys: [B, Hq, Tq, Tk] by strides */
+  const float* score;            /* optional, over the own keys */
+  const int32_t* lengths;        /* optional [B]: own keys that exist (clamped to [0, Tk]); those past it
+                                    are not read */
+  const float* kw_in;            /* optional [B, Hk, Tk] fp32 by strides (key axis contiguous) */
+  float* kw_out;                 /* optional output [B, Hk, Tk] fp32 contiguous */
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int64_t pk_stride_t, pk_stride_h, pv_stride_t, pv_stride_h;
+  int64_t k_stride_b, k_stride_t, k_stride_h;
+  int64_t v_stride_b, v_stride_t, v_stride_h;
+  int64_t o_stride_b, o_stride_t, o_stride_h;
+  int64_t o_lo_stride_b, o_lo_stride_t, o_lo_stride_h;
+  int64_t mask_stride_b, mask_stride_h, mask_stride_q;
+  int64_t score_stride_b, score_stride_h, score_stride_q;
+  int64_t kw_stride_b, kw_stride_h;
+  int32_t batch, seqlen_q, seqlen_p, seqlen_k, heads_q, heads_k, head_dim;
+  int32_t head_dim_in;           /* as in FaFwdParams */
+  float scale;
+  int32_t is_causal;             /* keep own key j for row i iff j <= i */
+  int32_t dtype;
+  void* stream;
+  void* workspace;               /* fa_prefix_plan bytes, 16-byte aligned, uninitialised */
+  int64_t workspace_bytes;
+  const void* mask_ws;           /* the prepared mask (fa_mask_prepare of this mask); required with a mask when
+                                    plan.needs_mask_ws */
+} FaPrefixParams;
+
+typedef struct FaPrefixPlan {
+  int32_t few_rows;              /* 1: rows packed in blocks of 32, the prefix read once for the batch; kw_out and
+                                    lengths are taken.  0: the 256-row blocks of fa_fwd for both key sets;
+                                    neither is (lengths as part of the mask, fa_key_weights for the weights) */
+  int32_t prefix_split;          /* key ranges of the prefix */
+  int32_t own_split;             /* key ranges of the own keys */
+  int32_t needs_mask_ws;         /* 1: a mask needs its prepared workspace (mask_ws) */
+  int64_t workspace_bytes;       /* size of FaPrefixParams.workspace */
+} FaPrefixPlan;
+
+/* From sizes, head dims, dtype, is_causal, and whether mask / score / kw_out are non-NULL. */
+int fa_prefix_plan(const FaPrefixParams* p, FaPrefixPlan* plan);
+int fa_prefix_fwd(const FaPrefixParams* p);
+
+/* Key weights of many rows: kw_out = kw_in + sum over the rows i of the kv-head's group of
+ * exp2(log2(e) scale (q_i k_j + score_ij) - lse_i) over kept keys, from the LSE that a forward
+ * left (over all keys of the row, a prefix among them). */
+typedef struct FaKeyWeightsParams {
+  const void* q;                 /* [B, Tq, Hq, D] */
+  const void* k;                 /* [B, Tk, Hk, D] */
+  const float* lse;              /* [B, Hq, Tq] */
+  const uint8_t* mask; const float* score; const int32_t* lengths;
+  const float* kw_in; float* kw_out;
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int64_t k_stride_b, k_stride_t, k_stride_h;
+  int64_t mask_stride_b, mask_stride_h, mask_stride_q;
+  int64_t score_stride_b, score_stride_h, score_stride_q;
+  int64_t kw_stride_b, kw_stride_h;
+  int32_t batch, seqlen_q, seqlen_k, heads_q, heads_k, head_dim, head_dim_in;
+  float scale;
+  int32_t is_causal;
+  int32_t dtype;
+  void* stream;
+  void* workspace;               /* fa_key_weights_plan bytes, 16-byte aligned, uninitialised */
+  int64_t workspace_bytes;
+} FaKeyWeightsParams;
+int fa_key_weights_plan(const FaKeyWeightsParams* p, int64_t* workspace_bytes);
+int fa_key_weights(const FaKeyWeightsParams* p);
+
+/* Eviction.  Of the n = lengths[b] (or Tk) keys of a sequence each kv-head keeps the last
+ * min(recent, n) and, of the others, those with the largest weight (ties: the lowest index; NaN
+ * above all) up to keep in all; n <= keep: all of them.  Outputs hold the kept keys in ascending
+ * order of their index; places behind the last one are zeros, with index -1. */
+typedef struct FaEvictParams {
+  const void* k; const void* v;  /* [B, Tk, Hk, D] by strides, 16-bit values */
+  const float* kw;               /* [B, Hk, Tk] by strides (key axis contiguous) */
+  const int32_t* lengths;        /* optional [B] (clamped to [0, Tk]) */
+  void* k_out; void* v_out;      /* [B, keep, Hk, D] by strides */
+  float* kw_out;                 /* [B, Hk, keep] contiguous */
+  int64_t* index_out;            /* [B, Hk, keep] contiguous */
+  int64_t k_stride_b, k_stride_t, k_stride_h;
+  int64_t v_stride_b, v_stride_t, v_stride_h;
+  int64_t kw_stride_b, kw_stride_h;
+  int64_t out_stride_b, out_stride_t, out_stride_h;   /* of k_out and v_out */
+  int32_t batch, seqlen_k, heads_k, head_dim;
+  int32_t keep;                  /* 1 .. seqlen_k */
+  int32_t recent;                /* 0 .. keep */
+  void* stream;
+} FaEvictParams;
+int fa_evict(const FaEvictParams* p);
+
+/* Rotary positions.  Column pair i < rotary / 2 of token (b, t) turns by the angle
+ * positions[axis(i), b, t] * inv_freq[i] (taken modulo 2 pi exactly, whatever the position);
+ * axis a owns the next sections[a] pairs.  Pair i is columns (i, i + rotary / 2), or with
+ * adjacent (2 i, 2 i + 1); columns from rotary on are copied.  sign -1 turns back (the
+ * gradient). */
+enum { FA_ROTARY_AXES = 8 };
+typedef struct FaRotaryParams {
+  const void* q; const void* k;  /* [B, T, Hq, D], [B, T, Hk, D]: any strides, columns contiguous */
+  void* q_out; void* k_out;
+  const void* positions;         /* [axes, B, T] by strides, int64 or int32 */
+  const float* inv_freq;         /* [rotary / 2] contiguous */
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int64_t k_stride_b, k_stride_t, k_stride_h;
+  int64_t qo_stride_b, qo_stride_t, qo_stride_h;
+  int64_t ko_stride_b, ko_stride_t, ko_stride_h;
+  int64_t pos_stride_a, pos_stride_b, pos_stride_t;
+  int32_t batch, seqlen, heads_q, heads_k, head_dim, rotary;
+  int32_t axes, sections[FA_ROTARY_AXES];
+  int32_t positions_64;          /* 1: int64, 0: int32 */
+  int32_t adjacent;
+  int32_t sign;                  /* 1 or -1 */
+  int32_t dtype;
+  void* stream;
+} FaRotaryParams;
+int fa_rotary(const FaRotaryParams* p);
 
 /* Human-readable description of the last nonzero status on the calling thread. */
 const char* fa_last_error(void);
