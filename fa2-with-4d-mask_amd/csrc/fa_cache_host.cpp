@@ -59,9 +59,35 @@ Tensor first_columns(const Tensor& x, int64_t D, bool bhsd) {
   return bhsd ? x.narrow(3, 0, D).transpose(1, 2).contiguous().transpose(1, 2) : x.narrow(3, 0, D).contiguous();
 }
 
-// A mask or score as [B|1, Hq|1, Tq, Tk] of its type with a contiguous key axis.
-Tensor side(const Tensor& x, at::ScalarType t) {
+// What the Python wrappers have checked, again: the custom ops can be called without them.
+void check_like(const Tensor& x, const Tensor& first, const char* name) {
+  TORCH_CHECK(x.dim() == 4 && x.device() == first.device() && x.scalar_type() == first.scalar_type(), name,
+              " must be a rank-4 tensor of the first operand's type and device");
+}
+void check_operands(const Tensor& q, const Tensor& k, const Tensor& v) {
+  TORCH_CHECK(q.is_cuda() && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf), "fp16 or bf16 GPU tensors expected");
+  check_like(q, q, "q");
+  check_like(k, q, "k");
+  check_like(v, q, "v");
+  TORCH_CHECK(v.sizes().equals(k.sizes()) && k.size(0) == q.size(0) && k.size(3) == q.size(3) && q.size(3) <= 256,
+              "q, k and v do not fit together, or the head dimension exceeds 256");
+}
+void check_lengths(const Tensor& n, const Tensor& first, int64_t B) {
+  TORCH_CHECK(!n.defined() || (n.scalar_type() == at::kInt && n.dim() == 1 && n.size(0) == B && n.is_contiguous() &&
+                               n.device() == first.device()),
+              "lengths must be a contiguous int32 tensor of the batch size on the operands' device");
+}
+void check_sums(const Tensor& w, const Tensor& first, int64_t B, int64_t H, int64_t T) {
+  TORCH_CHECK(!w.defined() || (w.scalar_type() == at::kFloat && w.sizes().equals({B, H, T}) && w.device() == first.device()),
+              "key weights must be a float32 tensor [batch, key heads, keys] on the operands' device");
+}
+
+// A mask or score [B|1, Hq|1, Tq, Tk] of its type with a contiguous key axis.
+Tensor side(const Tensor& x, at::ScalarType t, const Tensor& first, int64_t B, int64_t H, int64_t Tq, int64_t Tk) {
   if (!x.defined()) return x;
+  TORCH_CHECK(x.dim() == 4 && (x.size(0) == 1 || x.size(0) == B) && (x.size(1) == 1 || x.size(1) == H) && x.size(2) == Tq &&
+                  x.size(3) == Tk && x.device() == first.device(),
+              "a mask or score must be [batch or 1, heads or 1, rows, keys] on the operands' device");
   Tensor y = x.scalar_type() == t ? x : x.to(t);
   return y.size(3) == 1 || y.stride(3) == 1 ? y : y.contiguous();
 }
@@ -89,7 +115,7 @@ Tensor key_weights(const Tensor& q_, const Tensor& k_, const Tensor& lse_, const
   const int64_t D = q_.size(3), W = columns(D);
   const Tensor q = addressable(q_, bhsd, W), k = addressable(k_, bhsd, W), lse = lse_.contiguous();
   const Operand oq = operand(q, bhsd), ok = operand(k, bhsd);
-  const Tensor mask = side(get(mask_), at::kBool), score = side(get(score_), at::kFloat), lengths = get(lengths_);
+  const Tensor mask = get(mask_), score = get(score_), lengths = get(lengths_);
   FaKeyWeightsParams p{};
   set_sides(p, mask, score, lengths);
   p.q = oq.p; p.k = ok.p; p.lse = lse.const_data_ptr<float>();
@@ -123,11 +149,16 @@ Tensor key_weights(const Tensor& q_, const Tensor& k_, const Tensor& lse_, const
   return out;
 }
 
-// The own keys' mask with `lengths` as part of it, for kernels that take none: rows broadcast.
-Tensor with_lengths(const Tensor& mask, const Tensor& lengths, int64_t B, int64_t Tq, int64_t Tk) {
-  if (!lengths.defined()) return mask;
-  const Tensor keep = at::arange(Tk, lengths.options()).lt(lengths.view({B, 1, 1, 1})).expand({B, 1, Tq, Tk});
+// For kernels that take no lengths and read whole tiles: the own keys' mask with `lengths` as
+// part of it (rows broadcast), and K or V with zeros past them (0 times what stands there
+// would be NaN if that is no number).
+Tensor existing_keys(const Tensor& lengths, int64_t B, int64_t Tk) { return at::arange(Tk, lengths.options()).lt(lengths.view({B, 1})); }
+Tensor with_lengths(const Tensor& mask, const Tensor& there, int64_t B, int64_t Tq, int64_t Tk) {
+  const Tensor keep = there.view({B, 1, 1, Tk}).expand({B, 1, Tq, Tk});
   return mask.defined() ? mask.logical_and(keep) : keep;
+}
+Tensor zeros_past(const Tensor& x, const Tensor& there, bool bhsd) {
+  return at::where(bhsd ? there.view({there.size(0), 1, -1, 1}) : there.view({there.size(0), -1, 1, 1}), x, at::zeros({}, x.options()));
 }
 
 // O (in the caller's layout), LSE [B, Hq, Tq], O's rounding residual (empty unless asked for), key
@@ -137,6 +168,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor
                                                   const MaybeTensor& score_, const MaybeTensor& kw_, double scale, bool causal,
                                                   bool weights, bool residual, bool bhsd) {
   at::AutoDispatchBelowADInplaceOrView below;
+  check_operands(q_, k_, v_);
   const c10::DeviceGuard on_device(q_.device());
   RECORD_FUNCTION("tilelang_fa2_4d_mask::prefix_fwd", c10::ArrayRef<const c10::IValue>());
   const int t = bhsd ? 2 : 1, h = bhsd ? 1 : 2;
@@ -151,8 +183,18 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor
   p.is_causal = causal;
   p.dtype = dtype_code(q_);
   p.stream = stream_of(q_);
-  Tensor mask = Tk ? side(get(mask_), at::kBool) : Tensor(), lengths = Tk ? get(lengths_) : Tensor();
-  const Tensor score = Tk ? side(get(score_), at::kFloat) : Tensor();
+  if (Tp > 0) {
+    check_like(*pk_, q_, "pk");
+    TORCH_CHECK(pv_, "pk without pv");
+    check_like(*pv_, q_, "pv");
+    TORCH_CHECK(pv_->sizes().equals(pk_->sizes()) && pk_->size(0) == 1 && pk_->size(h) == Hk && pk_->size(3) == D,
+                "pk and pv do not fit k");
+  }
+  check_lengths(get(lengths_), q_, B);
+  check_sums(get(kw_), q_, B, Hk, Tk);
+  const Tensor own_mask = Tk ? side(get(mask_), at::kBool, q_, B, Hq, Tq, Tk) : Tensor();
+  Tensor mask = own_mask, lengths = Tk ? get(lengths_) : Tensor();
+  const Tensor score = Tk ? side(get(score_), at::kFloat, q_, B, Hq, Tq, Tk) : Tensor();
   set_sides(p, mask, score, lengths);
   const bool kw_too = weights && Tk > 0;
   Tensor kw = get(kw_), kw_out = at::empty({weights ? B : 0, Hk, Tk}, q_.options().dtype(at::kFloat));
@@ -163,14 +205,18 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor
     p.kw_out = nullptr;
     check(g_api.prefix_plan(&p, &plan), "fa_prefix_plan");
   }
+  Tensor k_clean = k_, v_clean = v_;
   if (!plan.few_rows && lengths.defined()) {
-    mask = with_lengths(mask, lengths, B, Tq, Tk);
+    const Tensor there = existing_keys(lengths, B, Tk);
+    mask = with_lengths(mask, there, B, Tq, Tk);
+    k_clean = zeros_past(k_, there, bhsd);
+    v_clean = zeros_past(v_, there, bhsd);
     p.lengths = nullptr;
     set_sides(p, mask, score, Tensor());
     check(g_api.prefix_plan(&p, &plan), "fa_prefix_plan");
   }
 
-  const Tensor q = addressable(q_, bhsd, W), k = addressable(k_, bhsd, W), v = addressable(v_, bhsd, W);
+  const Tensor q = addressable(q_, bhsd, W), k = addressable(k_clean, bhsd, W), v = addressable(v_clean, bhsd, W);
   const Operand oq = operand(q, bhsd), ok = operand(k, bhsd), ov = operand(v, bhsd);
   p.q = oq.p; p.k = ok.p; p.v = ov.p;
   p.q_stride_b = oq.sb; p.q_stride_t = oq.st; p.q_stride_h = oq.sh;
@@ -222,7 +268,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor
   p.workspace = ws.data_ptr();
   p.workspace_bytes = plan.workspace_bytes;
   check(g_api.prefix_fwd(&p), "fa_prefix_fwd");
-  if (kw_too && !p.kw_out) kw_out = key_weights(q, k, lse, get_opt(lengths), mask_, get_opt(score), kw_, scale, causal, bhsd);
+  if (kw_too && !p.kw_out) kw_out = key_weights(q, k, lse, get_opt(lengths), get_opt(own_mask), get_opt(score), kw_, scale, causal, bhsd);
   return {first_columns(out, D, bhsd), lse, residual ? first_columns(lo, D, bhsd) : at::empty({0}, q.options()), kw_out};
 }
 
@@ -232,6 +278,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> evict(const Tensor& k_, const Tensor&
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard on_device(k_.device());
   RECORD_FUNCTION("tilelang_fa2_4d_mask::evict", c10::ArrayRef<const c10::IValue>());
+  check_operands(k_, k_, v_);
+  check_lengths(get(lengths_), k_, k_.size(0));
+  check_sums(kw_, k_, k_.size(0), k_.size(bhsd ? 1 : 2), k_.size(bhsd ? 2 : 1));
+  TORCH_CHECK(keep >= 1 && keep <= k_.size(bhsd ? 2 : 1), "keep must lie in [1, keys]");
   auto rows = [](const Tensor& x) { return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous(); };
   const Tensor k = rows(k_), v = rows(v_), kw = key_axis_contiguous(kw_), lengths = get(lengths_);
   const Operand ok = operand(k, bhsd), ov = operand(v, bhsd);
@@ -259,6 +309,15 @@ using Pair = std::tuple<Tensor, Tensor>;
 
 Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Tensor& freq, const std::vector<int64_t>& sections,
                 bool adjacent, bool inverse, bool bhsd) {
+  check_operands(q_, k_, k_);
+  TORCH_CHECK(k_.size(bhsd ? 2 : 1) == q_.size(bhsd ? 2 : 1), "q and k do not fit together");
+  TORCH_CHECK(pos.dim() == 3 && (pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) && pos.device() == q_.device() &&
+                  pos.size(0) == (int64_t)sections.size() && (pos.size(1) == 1 || pos.size(1) == q_.size(0)) &&
+                  pos.size(2) == q_.size(bhsd ? 2 : 1),
+              "positions must be an int32 or int64 tensor [axes, batch or 1, tokens] on the operands' device");
+  TORCH_CHECK(freq.dim() == 1 && freq.scalar_type() == at::kFloat && freq.is_contiguous() && freq.device() == q_.device() &&
+                  freq.size(0) >= 1 && 2 * freq.size(0) <= q_.size(3),
+              "inv_freq must be a contiguous float32 vector on the operands' device");
   const c10::DeviceGuard on_device(q_.device());
   RECORD_FUNCTION("tilelang_fa2_4d_mask::rotary", c10::ArrayRef<const c10::IValue>());
   auto rows = [](const Tensor& x) { return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous(); };

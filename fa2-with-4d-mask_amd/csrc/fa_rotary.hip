@@ -2,8 +2,8 @@
 // positions[axis(i), b, t] * freq[i], queries and keys in one launch.
 //
 // The angle: freq / 2 pi as a 64-bit binary fraction of a turn, times the position modulo
-// 2^64.  Whole turns fall off by themselves and the rest is good to 2^-32 of a turn at any
-// position (a product in fp32 has lost 0.06 rad at position 10^6).  Cosines and sines are made
+// 2^64.  Whole turns fall off by themselves and the rest is good to 2^-31 of a turn at positions
+// below 2^32 (a product in fp32 has lost 0.06 rad at position 10^6).  Cosines and sines are made
 // once per token, into LDS, for all of its heads.
 //
 // What bounds it: reading and writing queries and keys once.
@@ -33,13 +33,18 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
     for (int e = 0; e < kRotaryAxes - 1; ++e) ax += e < a.naxes - 1 && i >= a.ends[e] ? 1 : 0;
     const int64_t at = ax * a.psa + b * a.psb + t * a.pst;
     const int64_t pos = a.pos64 ? ((const int64_t*)a.pos)[at] : ((const int32_t*)a.pos)[at];
-    const double turns = (double)a.freq[i] * 0.15915494309189533577;   // 1 / 2 pi
-    const double frac = turns - floor(turns);
-    const uint64_t turn = (uint64_t)(frac * 18446744073709551616.0);
-    const int32_t top = (int32_t)((turn * (uint64_t)pos) >> 32);       // in [-1/2, 1/2) turns, times 2^32
+    // freq / 2 pi in two doubles: 1 / 2 pi = kTurn + kTurnLo to 2^-110
+    constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnLo = -0x1.6b01ec5417056p-57;
+    const double f = (double)a.freq[i], turns = f * kTurn;
+    const double lo = fma(f, kTurnLo, fma(f, kTurn, -turns));
     float s, c;
-    sincospif((float)top * 0x1p-31f, &s, &c);
-    if (!(fabs(turns) < 1e300)) s = c = __builtin_nanf("");
+    if (fabs(turns) < 0x1p28) {
+      const uint64_t turn = (uint64_t)((turns - floor(turns)) * 0x1p64) + (uint64_t)(int64_t)rint(lo * 0x1p64);
+      const int32_t top = (int32_t)((turn * (uint64_t)pos) >> 32);   // in [-1/2, 1/2) turns, times 2^32
+      sincospif((float)top * 0x1p-31f, &s, &c);
+    } else {
+      s = c = __builtin_nanf("");   // no frequency: past 2^30, infinite or NaN
+    }
     cs[0][tk][i] = c;
     cs[1][tk][i] = s * a.sign;
   }

@@ -143,28 +143,13 @@ def _own_mask(mask, lengths, B: int, Tq: int, Tk: int):
     return keep if mask is None else mask & keep
 
 
-def _one_set_bwd(do, q, k, v, pk, pv, lengths, mask, score, o, lse, lo, scale, causal, atomic, bhsd):
-    """The gradients where there is only one key set, or no row: logical [B, T, H, D] in."""
-    B, Tq, Hq, _ = q.shape
-    Tk, Tp = k.shape[1], 0 if pk is None else _bthd(pk, bhsd).shape[1]
-    ws = torch.empty((0,), dtype=torch.uint8, device=q.device)
-    bwd = torch.ops.tilelang_fa2_4d_mask.bwd
-    dpk = dpv = q.new_empty((0,))
-    if Tp > 0 and Tk == 0 and B * Tq * Hq > 0:
-        one = [_one_sequence(x) for x in (do, q, o)]
-        lse1 = lse.transpose(0, 1).reshape(1, Hq, B * Tq).contiguous()
-        dq, dpk, dpv = bwd(one[0], one[1], _bthd(pk, bhsd), _bthd(pv, bhsd), one[2], lse1, None, None, ws,
-                           _one_sequence(lo) if lo.numel() else lo, scale, False, atomic)
-        dq, dk, dv = dq.view(q.shape), torch.zeros(k.shape, dtype=k.dtype, device=k.device), torch.zeros(
-            v.shape, dtype=v.dtype, device=v.device)
-        dpk, dpv = _bthd(dpk, bhsd), _bthd(dpv, bhsd)
-    elif Tk > 0 and B * Tq * Hq > 0:
-        dq, dk, dv = bwd(do, q, k, v, o, lse, _own_mask(mask, lengths, B, Tq, Tk), score, ws, lo, scale, causal, atomic)
-    else:
-        dq, dk, dv = (torch.zeros(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        if Tp > 0:
-            dpk, dpv = (_bthd(torch.zeros(_bthd(x, bhsd).shape, dtype=x.dtype, device=x.device), bhsd) for x in (pk, pv))
-    return _bthd(dq, bhsd), _bthd(dk, bhsd), _bthd(dv, bhsd), dpk, dpv
+def _existing(x: torch.Tensor, lengths) -> torch.Tensor:
+    """A logical [B, T, H, D] cache with zeros past the lengths, for kernels that read whole
+    tiles: 0 times what stands there would be NaN if that is no number."""
+    if lengths is None:
+        return x
+    there = torch.arange(x.shape[1], device=x.device) < lengths.view(-1, 1)
+    return torch.where(there[:, :, None, None], x, x.new_zeros(()))
 
 
 def _one_sequence(x: torch.Tensor) -> torch.Tensor:
@@ -230,32 +215,44 @@ def prefix_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     keys of both sets that point the same way); the prefix's pass takes the rows of the
     batch as one sequence, so that its dK and dV are summed over the batch in the kernel."""
     B, Tq, Tp, Tk, Hq, Hk, D = _sizes(q, k, pk, bhsd)
+
+    def zeros(x):
+        return _bthd(torch.zeros(_bthd(x, bhsd).shape, dtype=x.dtype, device=x.device), bhsd)
+
+    none = [q.new_empty((0,)), q.new_empty((0,))]
+    if B * Tq * Hq * D == 0 or Tp + Tk == 0:
+        return zeros(q), zeros(k), zeros(v), *((zeros(pk), zeros(pv)) if Tp else none)
     do, q, k, v, o = (_bthd(x, bhsd) for x in (do, q, k, v, o))
-    lo = _bthd(o_lo, bhsd) if o_lo.numel() else o_lo
-    if Tp == 0 or Tk == 0 or B * Tq * Hq == 0:
-        return _one_set_bwd(do, q, k, v, pk, pv, lengths, mask, score, o, lse, lo, scale, causal, atomic, bhsd)
-    pk, pv = _bthd(pk, bhsd), _bthd(pv, bhsd)
+    lo = _bthd(o_lo, bhsd) if o_lo.numel() else None
     _fa2._check_qkv(q, k, v)
-    _fa2._check_qkv(q, pk, pv)
-    if any(x.device != q.device for x in (o, lse, lo)) or o.dtype != q.dtype or lse.dtype != torch.float32:
+    if any(x is not None and x.device != q.device for x in (o, lse, lo)) or o.dtype != q.dtype or lse.dtype != torch.float32:
         raise ValueError("o, lse and o_lo must be on the device of q, o and lse as prefix_fwd returned them")
     op = _fa2._kernel_operand
-    q, k, v, pk, pv, o, lse = op(q), op(k), op(v), op(pk), op(pv), op(o), lse.contiguous()
-    lo = op(lo) if lo.numel() else None
-    m, mst = _fa2._kernel_side(_own_mask(mask, lengths, B, Tq, Tk), torch.bool, B, Hq, Tq, Tk, "mask", q.device)
-    s, sst = _fa2._kernel_side(score, torch.float32, B, Hq, Tq, Tk, "score", q.device)
     W = _fa2.kernel_head_dim(D)
-    # sums laid out [Hq, B Tq, W], which is [B, Hq, Tq, W] by strides for the own keys
-    sums = torch.empty((Hq, B * Tq, W), dtype=torch.float32, device=q.device)
-    _, dk, dv = _fa2._backward_impl(do, q, k, v, o, lse, m, s, None, mst, sst, scale, causal, atomic, lo,
-                                    (sums, _ext.FA_DQ_KEEP, Tq * W, B * Tq * W))
-    one = [_one_sequence(x) for x in (do, q, o)]
-    lse1 = lse.transpose(0, 1).reshape(1, Hq, B * Tq).contiguous()
-    lo1 = None if lo is None else op(_one_sequence(lo))
-    dq, dpk, dpv = _fa2._backward_impl(one[0], op(one[1]), pk, pv, op(one[2]), lse1, None, None, None, (0, 0, 0),
-                                       (0, 0, 0), scale, False, atomic, lo1, (sums, _ext.FA_DQ_ADD, 0, B * Tq * W))
-    dq = dq.view(B, Tq, Hq, D)
-    return tuple(_bthd(x, bhsd) for x in (dq, dk, dv, dpk, dpv))
+    # the sums laid out [Hq, B Tq, W], which is [B, Hq, Tq, W] by strides for the own keys
+    both = Tp > 0 and Tk > 0
+    sums = (torch.empty if both else torch.zeros)((Hq, B * Tq, W), dtype=torch.float32, device=q.device)
+    dk = dv = None
+    dpk, dpv = none
+    if Tk > 0:
+        m, mst = _fa2._kernel_side(_own_mask(mask, lengths, B, Tq, Tk), torch.bool, B, Hq, Tq, Tk, "mask", q.device)
+        s, sst = _fa2._kernel_side(score, torch.float32, B, Hq, Tq, Tk, "score", q.device)
+        dq, dk, dv = _fa2._backward_impl(
+            do, op(q), op(_existing(k, lengths)), op(_existing(v, lengths)), op(o), lse.contiguous(), m, s, None, mst, sst, scale,
+            causal, atomic, None if lo is None else op(lo), (sums, _ext.FA_DQ_KEEP if both else _ext.FA_DQ_ADD, Tq * W, B * Tq * W))
+    if Tp > 0:
+        pk, pv = _bthd(pk, bhsd), _bthd(pv, bhsd)
+        _fa2._check_qkv(q, pk, pv)
+        lse1 = lse.transpose(0, 1).reshape(1, Hq, B * Tq).contiguous()
+        dq, dpk, dpv = _fa2._backward_impl(
+            _one_sequence(do), op(_one_sequence(q)), op(pk), op(pv), op(_one_sequence(o)), lse1, None, None, None, (0, 0, 0),
+            (0, 0, 0), scale, False, atomic, None if lo is None else op(_one_sequence(lo)),
+            (sums, _ext.FA_DQ_ADD, 0, B * Tq * W))
+        dq = dq.view(B, Tq, Hq, D)
+        dpk, dpv = _bthd(dpk, bhsd), _bthd(dpv, bhsd)
+    if dk is None:
+        dk, dv = (torch.zeros(x.shape, dtype=x.dtype, device=x.device) for x in (k, v))
+    return _bthd(dq, bhsd), _bthd(dk, bhsd), _bthd(dv, bhsd), dpk, dpv
 
 
 @prefix_bwd.register_fake
@@ -526,10 +523,11 @@ def tilelang_rotary_embedding(
 
     query [B, Hq, T, D], key [B, Hk, T, D] (``layout="bshd"``: heads and tokens exchanged),
     fp16 / bf16, D up to 256.  positions: int32 / int64 [axes, B|1, T], any integers.
-    inv_freq: float32 [R / 2], R <= D the rotary columns; columns from R on are copied.
+    inv_freq: float32 [R / 2], R <= D the rotary columns; columns from R on are copied
+    (entries of 2^30 and more, infinite ones and NaN turn their pair into NaN).
     sections: how many of the R / 2 pairs turn with each axis, in order (None: one axis).
-    Pair i turns by ``positions[axis(i), b, t] * inv_freq[i]``, reduced exactly whatever the
-    position; it is columns (i, i + R / 2), or (2 i, 2 i + 1) with ``interleaved``:
+    Pair i turns by ``positions[axis(i), b, t] * inv_freq[i]``, multiplied in 64-bit fixed
+    point and reduced exactly (off by less than 2^-31 of a turn while |position| < 2^32); it is columns (i, i + R / 2), or (2 i, 2 i + 1) with ``interleaved``:
     ``(a, b) -> (a cos - b sin, b cos + a sin)``.
     Differentiable in query and key.  Returns new tensors (query, key) in the input layout.
     """

@@ -18,6 +18,9 @@ Contents
                (precision_check.py:110-130 and the config text).
 ``bruteforce`` float64 scalar-loop attention used to pin ``eager`` on tiny
                inputs.
+``cache``      definitions in 64 bits of the K/V cache operators (shared prefixes,
+               key weights, eviction, rotary positions), which the reference does
+               not have, and what their results may be off by.
 
 Parity status of each function is stated in its docstring ("pinned by ...").
 """
