@@ -60,7 +60,9 @@ struct EvictArgs {
   int64_t ksb, kst, ksh, vsb, vst, vsh, kwsb, kwsh, osb, ost, osh;
   int B, Tk, Hk, D, keep, recent;
   int vec;              // rows of 16-byte pieces, aligned
+  int nw;               // workgroups per (sequence, kv-head), each with ceil(keep / nw) places
 };
+constexpr int kEvictShare = 2048;   // most places of a workgroup
 hipError_t launch_evict(const EvictArgs& a, hipStream_t s);
 
 constexpr int kRotaryAxes = 8;

@@ -3,173 +3,241 @@
 // Of a sequence's n keys each kv-head keeps the last `recent` and, of the others, the need =
 // keep - recent with the largest weight, ties to the lowest index, in ascending order.
 //
-//   select_kernel  a workgroup per (sequence, kv-head).  Weights become unsigned integers of
-//                  the same order; the need-th largest is found digit by digit (11, 11, 10 bits:
-//                  a histogram of the digit among the values that agree so far, then the bin
-//                  the need-th falls into), then one scan in index order writes the kept indices
-//                  and weights.
-//   gather_kernel  copies the kept rows of K and V, a 16-byte piece per thread: it moves the
-//                  bytes that are kept, once.
+//   evict_kernel  a.nw workgroups of 16 waves per (sequence, kv-head).  Each finds the whole
+//                 selection: weights become unsigned integers of the same order; the need-th
+//                 largest is found digit by digit (12, 10, 10 bits: a histogram of the digit among
+//                 the values that agree so far, then the bin the need-th falls into); one pass in
+//                 index order then counts the kept keys.  Each copies its share of the kept rows
+//                 of K and V.
+//
+// The selection is a chain of dependent steps on little data (64 KB of weights for 16384 keys):
+// its latency counts, not its work, so that every workgroup of a head repeats it rather than wait
+// for one that writes indices to memory and for a second launch to read them.  The weights stay in
+// LDS, a stretch of 64-key pieces per wave; the order within a wave comes from ballots.  The copies move the bytes that are kept, once, 16 bytes per lane.
 #include "fa_cache.h"
 #include "fa_common.h"
 
 namespace fa {
 namespace {
 
-constexpr int kThreads = 1024, kBins = 2048;
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 4096;
 
 __device__ __forceinline__ int own_length(const EvictArgs& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
 }
 
-// Larger weights to larger integers; -0 as 0, every NaN above +inf.
+// Larger weights to larger integers; -0 as 0, every NaN above +inf.  No weight's is 0 or
+// kKept, the order of the most recent keys, above all.
+constexpr uint32_t kKept = ~0u;
 __device__ __forceinline__ uint32_t order(float w) {
-  if (w != w) return ~0u;
   const uint32_t u = __float_as_uint(w + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t x = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return w != w ? kKept - 1 : x;
 }
 
-// Sum of x over the lanes below this one, of the workgroup; *total: of all.
-__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* sums, uint32_t* total) {
+// Sum of x over the lanes up to this one (data moved between lanes by the VALU, not through LDS).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8: rows of 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // lane 15 of a row to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to rows 2 and 3
+  return x;
+}
+
+// Sum of x over the threads below this one, of the workgroup.
+__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t v = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(v, d);
-    if (lane >= d) v += y;
-  }
-  __syncthreads();   // (sums may still be read)
-  if (lane == 63) sums[wave] = v;
+  const uint32_t v = wave_scan(x);
+  if (lane == 63) sums[wave] = v;   // (last read before the barrier that ended the step before)
   __syncthreads();
-  uint32_t before = 0, all = 0;
+  uint32_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    const uint32_t y = sums[w];
-    before += w < wave ? y : 0;
-    all += y;
-  }
-  *total = all;
+  for (int w = 0; w < kWaves; ++w) before += w < wave ? sums[w] : 0;
   return before + v - x;
 }
 
-__global__ __launch_bounds__(kThreads) void select_kernel(const EvictArgs a) {
-  __shared__ uint32_t hist[kBins], sums[kThreads / 64], found[2];
-  const int bk = blockIdx.x, b = bk / a.Hk, kvh = bk - b * a.Hk;
-  const int tid = threadIdx.x;
+// CAP: weights of a cache that LDS holds (n <= CAP); 0: any number, read again for each step.
+// The loops over them stay rolled: unrolled over registers (32 pieces a lane) every step was new
+// code, run once, and the instruction fetches took 7 us a step.
+template <int CAP, bool VEC>
+__global__ __launch_bounds__(kThreads) void evict_kernel(const EvictArgs a) {
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
+  __shared__ uint32_t sums[kWaves], found[2];
+  __shared__ int list[kEvictShare];
+  __shared__ uint32_t keys[CAP > 0 ? CAP : 1];
+  const int bk = blockIdx.x / a.nw, part = blockIdx.x - bk * a.nw;
+  const int b = bk / a.Hk, kvh = bk - b * a.Hk;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* w = a.kw + b * a.kwsb + kvh * a.kwsh;
-  int64_t* idx = a.idx + (int64_t)bk * a.keep;
-  float* kwo = a.kwo + (int64_t)bk * a.keep;
   const int n = own_length(a, b);
   const int last = max(0, n - a.recent);             // keys [last, n) are kept whatever their weight
-  const int need = min(a.keep, n) - (n - last);      // of the keys [0, last)
-  // thr: keys above it are kept, and `ties` of those equal to it
-  uint32_t thr = 0, ties = 0;
-  if (need >= last) {
-    thr = 0;
-    ties = last;        // all (order() of no weight but -NaN is 0; equal ones count as ties)
-  } else if (need == 0) {
-    thr = ~0u;
-    ties = 0;
-  } else {
-    uint32_t known = 0, left = need;   // the left-th largest of those whose high digits are `thr`'s
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-      __syncthreads();
-      for (int j = tid; j < last; j += kThreads) {
-        const uint32_t u = order(w[j]);
-        if ((u & known) == (thr & known)) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1u);
+  // this wave's stretch: pieces [0, np) of 64 keys from k0 on
+  constexpr int U = 4;
+  const int np = ((n + kThreads - 1) / kThreads + U - 1) / U * U, k0 = wave * np * 64;
+  auto order_at = [&](int j, float x) __attribute__((always_inline)) -> uint32_t {
+    return j < last ? order(x) : (j < n ? kKept : 0u);
+  };
+  if constexpr (CAP > 0) {   // (each wave reads what it wrote; np <= CAP / 1024)
+#pragma unroll 4
+    for (int i = 0; i < np; i += U) {
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = w[min(k0 + (i + u) * 64 + lane, n - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = k0 + (i + u) * 64 + lane;
+        keys[j] = order_at(j, x[u]);
       }
+    }
+  }
+  // fn(key, its order) for every piece, in order
+  auto pieces = [&](auto&& fn) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int i = 0; i < np; i += U) {
+      uint32_t x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = k0 + (i + u) * 64 + lane;
+        if constexpr (CAP > 0) x[u] = keys[j];
+        else x[u] = order_at(j, w[min(j, n - 1)]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) fn(k0 + (i + u) * 64 + lane, x[u]);
+    }
+  };
+  // keys above thr are kept, and `ties` of those equal to it
+  uint32_t thr = 0, ties = 0;
+  if (n - last == a.keep) {
+    thr = kKept - 1;                     // the most recent ones alone
+  } else if (n > a.keep) {
+    // the left-th largest weight of those whose high digits are `thr`'s
+    uint32_t known = 0, left = a.keep - (n - last);
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 20 : (pass == 1 ? 10 : 0);
+      const uint32_t digit = pass == 0 ? 0xfffu : 0x3ffu;
+      *(u32x4*)(hist + 4 * tid) = u32x4{0, 0, 0, 0};
       __syncthreads();
-      // bins from the top: thread t has bins kBins - 1 - 2 t and the one below
-      const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
-      uint32_t total;
-      const uint32_t above = scan_before(hi + lo, sums, &total);
-      if (above < left && left <= above + hi + lo) {
-        const bool top = left <= above + hi;
-        found[0] = kBins - 1 - 2 * tid - (top ? 0 : 1);
-        found[1] = left - above - (top ? 0 : hi);
+      pieces([&](int, uint32_t u) __attribute__((always_inline)) {
+        // (weights only: keys past n, and the most recent ones, would all meet in one bin)
+        if (u - 1 < kKept - 1 && ((u ^ thr) & known) == 0) atomicAdd(&hist[(u >> shift) & digit], 1u);
+      });
+      __syncthreads();
+      // bins from the top: thread t has the four from kBins - 1 - 4 t down
+      const u32x4 h = *(const u32x4*)(hist + kBins - 4 - 4 * tid);
+      uint32_t above = scan_before((h[0] + h[1]) + (h[2] + h[3]), sums);
+      if (above < left && left <= above + (h[0] + h[1]) + (h[2] + h[3])) {
+        int bin = 3;
+        while (left > above + h[bin]) above += h[bin--];
+        found[0] = kBins - 4 - 4 * tid + bin;
+        found[1] = left - above;
       }
       __syncthreads();
       thr |= found[0] << shift;
       left = found[1];
-      known |= ((1u << bits) - 1) << shift;
-      __syncthreads();
+      known |= digit << shift;
     }
     ties = left;
   }
-  // ---- in index order: thread t's keys are [t per, (t + 1) per) ---------------------------
-  const int per = (n + kThreads - 1) / kThreads;
-  const int j0 = min(tid * per, n), j1 = min(j0 + per, n);
-  uint32_t eq = 0, gt = 0;
-  for (int j = j0; j < j1; ++j) {
-    if (j >= last) {
-      ++gt;
+  // ---- kept keys and ties of the waves' stretches, those before this one's added up -----------
+  uint32_t gt = 0, eq = 0;   // of the wave, the same in every lane
+  pieces([&](int, uint32_t u) __attribute__((always_inline)) {
+    gt += __popcll(__builtin_amdgcn_ballot_w64(u > thr));
+    eq += __popcll(__builtin_amdgcn_ballot_w64(u == thr));
+  });
+  const int share = (a.keep + a.nw - 1) / a.nw, i0 = part * share, i1 = min(i0 + share, a.keep);
+  for (int i = tid; i < share; i += kThreads) list[i] = -1;
+  __syncthreads();   // (hist is free)
+  if (lane == 0) {
+    hist[wave] = gt;
+    hist[kWaves + wave] = eq;
+  }
+  __syncthreads();
+  uint32_t before = 0, seen = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    before += i < wave ? hist[i] : 0;
+    seen += i < wave ? hist[kWaves + i] : 0;
+  }
+  // ---- this workgroup's places [i0, i1), filled by the waves whose keys go there ---------------
+  int at = (int)__builtin_amdgcn_readfirstlane(before + min(seen, ties)) - i0;
+  seen = __builtin_amdgcn_readfirstlane(seen);
+  const int end = at + (int)(gt + min(eq, ties - min(seen, ties)));
+  if (end > 0 && at < share) {
+    const uint64_t below = (1ull << lane) - 1;
+    pieces([&](int j, uint32_t u) __attribute__((always_inline)) {
+      bool kept = u > thr;
+      const uint64_t te = __builtin_amdgcn_ballot_w64(u == thr);
+      if (te != 0) {
+        kept = kept || (u == thr && seen + __popcll(te & below) < ties);
+        seen += __popcll(te);
+      }
+      const uint64_t ke = __builtin_amdgcn_ballot_w64(kept);
+      const int place = at + __popcll(ke & below);
+      if (kept && (uint32_t)place < (uint32_t)share) list[place] = j;
+      at += __popcll(ke);
+    });
+  }
+  __syncthreads();
+  const int64_t o0 = (int64_t)bk * a.keep;
+  for (int i = i0 + tid; i < i1; i += kThreads) {
+    const int j = list[i - i0];
+    a.idx[o0 + i] = j;
+    a.kwo[o0 + i] = j < 0 ? 0.f : w[j];
+  }
+  // ---- the rows -------------------------------------------------------------------------
+  const int CH = VEC ? a.D / 8 : a.D, rpp = max(kThreads / CH, 1), lanes = min(CH, kThreads);
+  const int r0 = tid / CH;
+  if (r0 >= rpp) return;
+  const uint16_t* kp = (const uint16_t*)a.k + b * a.ksb + kvh * a.ksh;
+  const uint16_t* vp = (const uint16_t*)a.v + b * a.vsb + kvh * a.vsh;
+  uint16_t* ko = (uint16_t*)a.ko + b * a.osb + kvh * a.osh;
+  uint16_t* vo = (uint16_t*)a.vo + b * a.osb + kvh * a.osh;
+  for (int ch = tid - r0 * CH; ch < CH; ch += lanes) {
+    const int c = ch * (VEC ? 8 : 1);
+    if constexpr (VEC) {
+      constexpr int U = 4;   // rows in flight
+      for (int i = i0 + r0; i < i1; i += U * rpp) {
+        u32x4 x[U], y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int j = i + u * rpp < i1 ? list[i + u * rpp - i0] : -1;
+          x[u] = gload16_if(j >= 0, kp + (int64_t)max(j, 0) * a.kst + c);
+          y[u] = gload16_if(j >= 0, vp + (int64_t)max(j, 0) * a.vst + c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i + u * rpp < i1) {
+            gstore16(ko + (int64_t)(i + u * rpp) * a.ost + c, x[u]);
+            gstore16(vo + (int64_t)(i + u * rpp) * a.ost + c, y[u]);
+          }
+      }
     } else {
-      const uint32_t u = order(w[j]);
-      gt += u > thr;
-      eq += u == thr;
+      for (int i = i0 + r0; i < i1; i += rpp) {
+        const int j = list[i - i0];
+        ko[(int64_t)i * a.ost + c] = j >= 0 ? kp[(int64_t)j * a.kst + c] : (uint16_t)0;
+        vo[(int64_t)i * a.ost + c] = j >= 0 ? vp[(int64_t)j * a.vst + c] : (uint16_t)0;
+      }
     }
-  }
-  uint32_t all;
-  const uint32_t eq_before = scan_before(eq, sums, &all);
-  const uint32_t eq_mine = min(eq, ties - min(ties, eq_before));
-  uint32_t at = scan_before(gt + eq_mine, sums, &all), seen = eq_before;
-  for (int j = j0; j < j1; ++j) {
-    bool kept = j >= last;
-    if (!kept) {
-      const uint32_t u = order(w[j]);
-      kept = u > thr || (u == thr && seen++ < ties);
-    }
-    if (kept) {
-      idx[at] = j;
-      kwo[at] = w[j];
-      ++at;
-    }
-  }
-  for (int i = (int)all + tid; i < a.keep; i += kThreads) {   // places behind the last key
-    idx[i] = -1;
-    kwo[i] = 0.f;
   }
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a) {
-  const int CH = VEC ? a.D / 8 : a.D;
-  const int64_t n = (int64_t)a.B * a.Hk * a.keep * CH;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < n; x += (int64_t)gridDim.x * 256) {
-    const int c = (int)(x % CH) * (VEC ? 8 : 1);
-    const int64_t row = x / CH;
-    const int i = (int)(row % a.keep), bk = (int)(row / a.keep);
-    const int b = bk / a.Hk, kvh = bk - b * a.Hk;
-    const int64_t j = a.idx[row];
-    const int64_t src_k = b * a.ksb + j * a.kst + kvh * a.ksh + c, src_v = b * a.vsb + j * a.vst + kvh * a.vsh + c;
-    const int64_t dst = b * a.osb + i * a.ost + kvh * a.osh + c;
-    if constexpr (VEC) {
-      u32x4 k = u32x4{0, 0, 0, 0}, v = k;
-      if (j >= 0) {
-        k = gload16((const uint16_t*)a.k + src_k);
-        v = gload16((const uint16_t*)a.v + src_v);
-      }
-      gstore16((uint16_t*)a.ko + dst, k);
-      gstore16((uint16_t*)a.vo + dst, v);
-    } else {
-      ((uint16_t*)a.ko)[dst] = j >= 0 ? ((const uint16_t*)a.k)[src_k] : (uint16_t)0;
-      ((uint16_t*)a.vo)[dst] = j >= 0 ? ((const uint16_t*)a.v)[src_v] : (uint16_t)0;
-    }
-  }
+template <int CAP> hipError_t launch_c(const EvictArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.B * a.Hk * a.nw)), block(kThreads);
+  if (a.vec) hipLaunchKernelGGL((evict_kernel<CAP, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((evict_kernel<CAP, false>), grid, block, 0, s, a);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(select_kernel, dim3((unsigned)(a.B * a.Hk)), dim3(kThreads), 0, s, a);
-  if (const hipError_t e = hipGetLastError()) return e;
-  const int64_t n = ((int64_t)a.B * a.Hk * a.keep * (a.vec ? a.D / 8 : a.D) + 255) / 256;
-  const dim3 grid((unsigned)min_i64(n, 1 << 20));
-  if (a.vec) hipLaunchKernelGGL((gather_kernel<true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((gather_kernel<false>), grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+  if (a.Tk <= 8192) return launch_c<8192>(a, s);
+  if (a.Tk <= 32768) return launch_c<32768>(a, s);
+  return launch_c<0>(a, s);
 }
 
 }  // namespace fa

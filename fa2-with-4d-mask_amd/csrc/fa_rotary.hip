@@ -56,58 +56,70 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   const int pc = tid % NP;
   int h = tid / NP, tk = 0;
   if (h >= step) return;
-  while (h >= H) {
-    h -= H;
-    ++tk;
-  }
-  typedef T TV __attribute__((ext_vector_type(V)));
-  while (tk < nt) {
-    const int64_t bt = tok0 + tk;
-    const int64_t b = bt / a.T, t = bt - b * a.T;
-    const bool isq = h < a.Hq;
-    const int hh = isq ? h : h - a.Hq;
-    const T* src = isq ? (const T*)a.q + b * a.qsb + t * a.qst + hh * a.qsh : (const T*)a.k + b * a.ksb + t * a.kst + hh * a.ksh;
-    T* dst = isq ? (T*)a.qo + b * a.qosb + t * a.qost + hh * a.qosh : (T*)a.ko + b * a.kosb + t * a.kost + hh * a.kosh;
-    if (pc >= NR) {
-      const int c = 2 * a.R2 + (pc - NR) * V;
-      *(TV*)(dst + c) = *(const TV*)(src + c);
-    } else if constexpr (ADJ) {
-      const int c = pc * V;
-      if constexpr (V == 1) {
-        const int i = c >> 1;
-        const float co = cs[0][tk][i], si = cs[1][tk][i];
-        const float x = (float)src[c], y = (float)src[c ^ 1];
-        dst[c] = (T)(c & 1 ? fmaf(x, co, y * si) : fmaf(x, co, -(y * si)));
-      } else {
-        const TV x = *(const TV*)(src + c);
-        TV y;
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          const float co = cs[0][tk][(c + e) >> 1], si = cs[1][tk][(c + e) >> 1];
-          const float u = (float)x[e], v = (float)x[e + 1];
-          y[e] = (T)fmaf(u, co, -(v * si));
-          y[e + 1] = (T)fmaf(v, co, u * si);
-        }
-        *(TV*)(dst + c) = y;
-      }
-    } else {
-      const int c = pc * V;
-      const TV x0 = *(const TV*)(src + c), x1 = *(const TV*)(src + a.R2 + c);
-      TV y0, y1;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float co = cs[0][tk][c + e], si = cs[1][tk][c + e];
-        const float u = (float)x0[e], v = (float)x1[e];
-        y0[e] = (T)fmaf(u, co, -(v * si));
-        y1[e] = (T)fmaf(v, co, u * si);
-      }
-      *(TV*)(dst + c) = y0;
-      *(TV*)(dst + a.R2 + c) = y1;
-    }
-    h += step;
+  auto settle = [&]() __attribute__((always_inline)) {
     while (h >= H) {
       h -= H;
       ++tk;
+    }
+  };
+  settle();
+  typedef T TV __attribute__((ext_vector_type(V)));
+  const bool turned = pc < NR;
+  const int c0 = turned ? pc * V : 2 * a.R2 + (pc - NR) * V;
+  const int c1 = ADJ ? (V == 1 && turned ? c0 ^ 1 : c0) : (turned ? c0 + a.R2 : c0);
+  // kFly pieces at a time: their loads go out together
+  constexpr int kFly = 4;
+  while (tk < nt) {
+    TV x0[kFly], x1[kFly];
+    T* dst[kFly];
+    int at[kFly];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      at[u] = tk;
+      if (tk < nt) {
+        const int64_t bt = tok0 + tk;
+        const int64_t b = bt / a.T, t = bt - b * a.T;
+        const bool isq = h < a.Hq;
+        const int hh = isq ? h : h - a.Hq;
+        const T* src = isq ? (const T*)a.q + b * a.qsb + t * a.qst + hh * a.qsh : (const T*)a.k + b * a.ksb + t * a.kst + hh * a.ksh;
+        dst[u] = isq ? (T*)a.qo + b * a.qosb + t * a.qost + hh * a.qosh : (T*)a.ko + b * a.kosb + t * a.kost + hh * a.kosh;
+        x0[u] = *(const TV*)(src + c0);
+        if (!ADJ || V == 1) x1[u] = *(const TV*)(src + c1);
+      }
+      h += step;
+      settle();
+    }
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      if (at[u] >= nt) continue;
+      if (!turned) {
+        *(TV*)(dst[u] + c0) = x0[u];
+      } else if constexpr (ADJ && V == 1) {
+        const float co = cs[0][at[u]][c0 >> 1], si = cs[1][at[u]][c0 >> 1];
+        const float x = (float)x0[u][0], y = (float)x1[u][0];
+        dst[u][c0] = (T)fmaf(x, co, c0 & 1 ? y * si : -(y * si));
+      } else if constexpr (ADJ) {
+        TV y;
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          const float co = cs[0][at[u]][(c0 + e) >> 1], si = cs[1][at[u]][(c0 + e) >> 1];
+          const float p = (float)x0[u][e], q = (float)x0[u][e + 1];
+          y[e] = (T)fmaf(p, co, -(q * si));
+          y[e + 1] = (T)fmaf(q, co, p * si);
+        }
+        *(TV*)(dst[u] + c0) = y;
+      } else {
+        TV y0, y1;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float co = cs[0][at[u]][c0 + e], si = cs[1][at[u]][c0 + e];
+          const float p = (float)x0[u][e], q = (float)x1[u][e];
+          y0[e] = (T)fmaf(p, co, -(q * si));
+          y1[e] = (T)fmaf(q, co, p * si);
+        }
+        *(TV*)(dst[u] + c0) = y0;
+        *(TV*)(dst[u] + c1) = y1;
+      }
     }
   }
 }
