@@ -26,12 +26,14 @@ struct PrefixArgs {
   int ctp, cto;         // 32-key tiles of each range (the last may have fewer)
   int nrbp, nrbo;       // 32-row blocks: of a kv-head's rows over the batch, of one sequence's
   int np, no;           // workgroups: prefix, own
+  int wide;             // the prefix in blocks of kWideRows rows (ctp counts 64-key tiles then)
   float* part_o;
   float* part_ml;
   float* logits;        // with kw_out: raw logits [rows][Tkp] of the own keys (-inf: dropped)
   int Tkp;
 };
 constexpr int kPrefixSlots = 128;     // most key ranges of a problem: two per lane of the joining wave
+constexpr int kWideRows = 128;
 constexpr int kPrefixKwRows = 64;     // most rows of a kv-head's group with kw_out
 int prefix_tile_keys();
 hipError_t launch_prefix_rows(const PrefixArgs& a, int D, int dtype, hipStream_t s);

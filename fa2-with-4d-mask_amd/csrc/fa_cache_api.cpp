@@ -73,7 +73,7 @@ void scales(float scale, float* scale_log2, float* qsign, int* zero) {
 constexpr int kFewRows = 32;
 
 struct PrefixPlan {
-  bool few;
+  bool few, wide;
   int ctp, cto, nsp, nso, nrbp, nrbo;
   int64_t np, no, rows, bytes;
   int Tkp;
@@ -97,20 +97,30 @@ PrefixPlan prefix_plan(const FaPrefixParams* p) {
     f.bytes = f.rows * (f.nsp + f.nso) * (p->head_dim + 2) * (int64_t)sizeof(float);
     return f;
   }
-  const int64_t rbp = ceil_div(TG * p->batch, 32), rbo = ceil_div(TG, 32);
-  const int64_t ntp = ceil_div(p->seqlen_p, kt), nto = ceil_div(p->seqlen_k, kt);
+  // The prefix in blocks of 128 rows sharing its 64-key tiles, where those give every CU four tiles;
+  // else in blocks of 32.  In us, wide / not (bf16, Hq 32, Hk 8, D 128, one row of B sequences):
+  // B24 Tp8192 20.7 / 23.1, B48 Tp8192 and 256 own 32.5 / 34.4, B32 Tp32000 54.3 / 64.4, B20 Tq16
+  // Hq16 Hk4 Tp4000 37 / 44; with less B32 Tp1000 17.4 / 16.4, B60 Hk1 D64 Tp4000 20.7 / 19.2.
+  const int64_t wide_tiles = p->heads_k * ceil_div(TG * p->batch, fa::kWideRows) * ceil_div(p->seqlen_p, 64);
+  f.wide = p->head_dim <= 128 && TG * p->batch > 64 && wide_tiles >= 4 * fa::kCus;
+  const int rows_p = f.wide ? fa::kWideRows : 32, keys_p = f.wide ? 64 : kt;
+  const int64_t rbp = ceil_div(TG * p->batch, rows_p), rbo = ceil_div(TG, 32);
+  const int64_t ntp = ceil_div(p->seqlen_p, keys_p), nto = ceil_div(p->seqlen_k, kt);
   const int64_t base_p = ntp ? p->heads_k * rbp : 0, base_o = nto ? (int64_t)p->batch * p->heads_k * rbo : 0;
-  // Tiles per range, the same for both key sets: as many ranges as two rounds of workgroups on
-  // the chip, but no less than a tile for every wave, and no more slots than the join holds.
+  // Tiles per range: one round of workgroups (two per CU; wide ones beside the own keys': one),
+  // four tiles for every wave where there are as many, no more slots than the join holds.
+  // (B16 Tp8192: ranges of 4 tiles 26.7 us, 16 16.9, 24 18.0; own keys of B64 Tk512 in two rounds 28.3, in
+  // one 24.8.)
   const int64_t slots = (p->head_dim > 128 ? 1 : 2) * fa::kCus;
-  const int64_t per = std::max<int64_t>(4, ceil_div(base_p * ntp + base_o * nto, 2 * slots));
-  auto ranges = [&](int64_t nt, int* ct) -> int {
+  const int64_t per = std::max<int64_t>(16, ceil_div((f.wide ? 0 : base_p * ntp) + base_o * nto, slots));
+  const int64_t per_p = f.wide ? std::max<int64_t>(4, ceil_div(wide_tiles, fa::kCus)) : per;
+  auto ranges = [&](int64_t nt, int64_t per, int* ct) -> int {
     const int64_t ns = std::min<int64_t>(fa::kPrefixSlots / 2, ceil_div(nt, per));
     *ct = ns ? (int)ceil_div(nt, ns) : 1;
     return ns ? (int)ceil_div(nt, *ct) : 0;
   };
-  f.nsp = ranges(ntp, &f.ctp);
-  f.nso = ranges(nto, &f.cto);
+  f.nsp = ranges(ntp, per_p, &f.ctp);
+  f.nso = ranges(nto, per, &f.cto);
   f.np = base_p * f.nsp;
   f.no = base_o * f.nso;
   f.nrbp = (int)rbp;
@@ -193,7 +203,7 @@ int fa_prefix_plan(const FaPrefixParams* p, FaPrefixPlan* plan) {
   if (const int st = check_prefix(p)) return st;
   if (!plan) return fail(FA_ERR_NULL, "plan is NULL");
   const PrefixPlan f = prefix_plan(p);
-  *plan = FaPrefixPlan{f.few && (!p->kw_out || kw_fits(p)) ? 1 : 0, f.nsp, f.nso, f.few ? 0 : 1, f.bytes};
+  *plan = FaPrefixPlan{f.few && (!p->kw_out || kw_fits(p)) ? 1 : 0, f.nsp, f.nso, f.few ? 0 : 1, f.bytes, f.wide ? 1 : 0, 0};
   return FA_OK;
 }
 
@@ -257,6 +267,7 @@ int fa_prefix_fwd(const FaPrefixParams* p) {
   a.mask4 = mask_by_words(p->mask, p->mask_stride_b, p->mask_stride_h, p->mask_stride_q);
   a.nsp = f.nsp; a.nso = f.nso; a.ctp = f.ctp; a.cto = f.cto; a.nrbp = f.nrbp; a.nrbo = f.nrbo;
   a.np = (int)f.np; a.no = (int)f.no;
+  a.wide = f.wide;
   a.part_o = (float*)p->workspace;
   a.part_ml = a.part_o + f.rows * (f.nsp + f.nso) * p->head_dim;
   a.logits = a.part_ml + f.rows * (f.nsp + f.nso) * 4;

@@ -161,9 +161,9 @@ Tensor zeros_past(const Tensor& x, const Tensor& there, bool bhsd) {
   return at::where(bhsd ? there.view({there.size(0), 1, -1, 1}) : there.view({there.size(0), -1, 1, 1}), x, at::zeros({}, x.options()));
 }
 
-// O (in the caller's layout), LSE [B, Hq, Tq], O's rounding residual (empty unless asked for), key
-// weights [B, Hk, Tk] (empty unless asked for).
-std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& pk_,
+// O (in the caller's layout), LSE [B, Hq, Tq], O's rounding residual and key weights [B, Hk, Tk]
+// (none unless asked for).
+std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& pk_,
                                                   const MaybeTensor& pv_, const MaybeTensor& lengths_, const MaybeTensor& mask_,
                                                   const MaybeTensor& score_, const MaybeTensor& kw_, double scale, bool causal,
                                                   bool weights, bool residual, bool bhsd) {
@@ -197,7 +197,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor
   const Tensor score = Tk ? side(get(score_), at::kFloat, q_, B, Hq, Tq, Tk) : Tensor();
   set_sides(p, mask, score, lengths);
   const bool kw_too = weights && Tk > 0;
-  Tensor kw = get(kw_), kw_out = at::empty({weights ? B : 0, Hk, Tk}, q_.options().dtype(at::kFloat));
+  Tensor kw = get(kw_), kw_out;
+  if (weights) kw_out = at::empty({B, Hk, Tk}, q_.options().dtype(at::kFloat));
   if (kw_too) p.kw_out = kw_out.data_ptr<float>();
   FaPrefixPlan plan{};
   check(g_api.prefix_plan(&p, &plan), "fa_prefix_plan");
@@ -269,7 +270,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attend(const Tensor& q_, const Tensor
   p.workspace_bytes = plan.workspace_bytes;
   check(g_api.prefix_fwd(&p), "fa_prefix_fwd");
   if (kw_too && !p.kw_out) kw_out = key_weights(q, k, lse, get_opt(lengths), get_opt(own_mask), get_opt(score), kw_, scale, causal, bhsd);
-  return {first_columns(out, D, bhsd), lse, residual ? first_columns(lo, D, bhsd) : at::empty({0}, q.options()), kw_out};
+  return {first_columns(out, D, bhsd), lse, residual ? MaybeTensor(first_columns(lo, D, bhsd)) : std::nullopt, get_opt(kw_out)};
 }
 
 // K, V and weights of the kept keys, and their indices.
@@ -366,11 +367,17 @@ struct Rotary : torch::autograd::Function<Rotary> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
     const auto s = ctx->get_saved_variables();
     const int64_t flags = ctx->saved_data["flags"].toInt();
-    auto r = Rotary::apply(g[0], g[1], s[0], s[1], ctx->saved_data["sections"].toIntVector(), (bool)(flags & 1),
-                           !(flags >> 1 & 1), (bool)(flags >> 2 & 1));
+    const std::vector<int64_t> sections = ctx->saved_data["sections"].toIntVector();
+    const bool adjacent = flags & 1, inverse = !(flags >> 1 & 1), bhsd = flags >> 2 & 1;
     torch::autograd::variable_list out(8);
-    out[0] = r[0];
-    out[1] = r[1];
+    if (at::GradMode::is_enabled()) {
+      auto r = Rotary::apply(g[0], g[1], s[0], s[1], sections, adjacent, inverse, bhsd);
+      out[0] = r[0];
+      out[1] = r[1];
+    } else {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(out[0], out[1]) = rotary_run(g[0], g[1], s[0], s[1], sections, adjacent, inverse, bhsd);
+    }
     return out;
   }
 };

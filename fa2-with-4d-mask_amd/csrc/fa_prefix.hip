@@ -380,11 +380,181 @@ __device__ __forceinline__ void rows_body(const PrefixArgs& a, const int W, char
   }
 }
 
+// The prefix for many rows (a.wide: at least kWideRows of a kv-head over the batch): 128 rows per
+// workgroup, 32 per wave, every wave walks all 64-key tiles of the range, which the workgroup
+// stages once in LDS (two buffers, one barrier per tile).  Against rows_body, whose waves have 32
+// rows in common and cut the keys: K and V come from memory once per 128 rows, two independent
+// chains of S products per wave hide each other's latency, and there is no merge.
+constexpr int kWideKeys = 64;
+// K rows are read 16 consecutive ones of a chunk at a time, V as 4 rows x 4 chunks.
+template <int D> __device__ __forceinline__ int swz_wk(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
+
+template <typename T, int D>
+__device__ __forceinline__ void wide_body(const PrefixArgs& a, const int W, char* smem) {
+  using V8 = typename Vec8<T>::type;
+  constexpr int DS = D / 16, NB = D / 32, CH = D / 8, ROWB = 2 * D;
+  constexpr int TB = kWideKeys * ROWB;             // bytes of a K or V tile
+  constexpr int U = kWideKeys * CH / (kWaves * 64);   // 16-byte chunks per thread and kind
+  const int nrb = a.nrbp;
+  const int rb = W % nrb, W1 = W / nrb;
+  const int sp = W1 % a.nsp, kvh = W1 / a.nsp;
+  const int TG = a.Tq * a.G, R = a.B * TG;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hf = lane >> 5;
+  const int row = rb * kWideRows + wave * 32 + l32;
+  const int r = min(row, R - 1);
+  const int b = r / TG, rr = r - b * TG, tq = rr / a.G, h = kvh * a.G + (rr - tq * a.G);
+  const float c2 = a.scale_log2;
+  const int Tk = a.Tp;
+
+  V8 qf[DS];
+  {
+    const uint32_t neg = a.qsign < 0.f ? 0x80008000u : 0u;
+    u32x4 x[DS];
+    load_row(x, (const T*)a.q + b * a.qsb + h * a.qsh + (int64_t)tq * a.qst + hf * 8, a.Dv);
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec8<T>(only_cols(x[ds], ds, a.Dv, neg));
+  }
+  const T* __restrict__ kp = (const T*)a.pk + kvh * a.pksh;
+  const T* __restrict__ vp = (const T*)a.pv + kvh * a.pvsh;
+  const int nt = (Tk + kWideKeys - 1) / kWideKeys;
+  const int t_lo = min(sp * a.ctp, nt), t_hi = min(t_lo + a.ctp, nt);
+
+  // staging: thread -> chunk c of tile row tr + u (256 / CH)
+  uint32_t gk[U], gv[U], lk[U], lv[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int idx = tid + u * kWaves * 64, tr = idx / CH, c = idx % CH;
+    gk[u] = 8 * c < a.Dv ? (uint32_t)(tr * a.pkst * 2) + (uint32_t)(c * 16) : kNoRec;
+    gv[u] = 8 * c < a.Dv ? (uint32_t)(tr * a.pvst * 2) + (uint32_t)(c * 16) : kNoRec;
+    lk[u] = tr * ROWB + ((c ^ swz_wk<D>(tr)) * 16);
+    lv[u] = TB + tr * ROWB + ((c ^ swz_v<D>(tr)) * 16);
+  }
+  u32x4 kr[U], vr[U];
+  auto rs_of = [&](const T* base, int64_t st, int t) __attribute__((always_inline)) {
+    const int rows = t < t_hi ? min(Tk - t * kWideKeys, kWideKeys) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (rows > 0 ? (int64_t)t * kWideKeys * st : 0)), (short)0,
+                                             rows > 0 ? (int)((int64_t)(rows - 1) * st * 2 + 2 * a.Dv) : 0, 0x00020000);
+  };
+  auto load = [&](int t) __attribute__((always_inline)) {   // (past the range: zeros)
+    const auto rk = rs_of(kp, a.pkst, t), rv = rs_of(vp, a.pvst, t);
+#pragma unroll
+    for (int u = 0; u < U; ++u) kr[u] = __builtin_amdgcn_raw_buffer_load_b128(rk, gk[u], 0, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) vr[u] = __builtin_amdgcn_raw_buffer_load_b128(rv, gv[u], 0, 0);
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {
+    char* p = smem + buf * 2 * TB;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      lds_write16(p + lk[u], kr[u]);
+      lds_write16(p + lv[u], vr[u]);
+    }
+  };
+
+  f32x16 oacc[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) oacc[nb] = f32x16{};
+  float m_run = kNegInf, l_run = 0.f;
+  const int tr_row = 4 * hf + ((lane >> 2) & 3);
+  const int tr_col = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+
+  if (t_lo < t_hi) {
+    load(t_lo);
+    store(0);
+    __syncthreads();
+  }
+  for (int t = t_lo; t < t_hi; ++t) {
+    const char* kt = smem + ((t - t_lo) & 1) * 2 * TB;
+    const char* vt = kt + TB;
+    load(t + 1);
+    f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int kr_ = kb * 32 + l32;
+        s[kb] = mfma32(as_vec8<T>(lds_read16(kt + kr_ * ROWB + (((2 * ds + hf) ^ swz_wk<D>(kr_)) * 16))), qf[ds], s[kb]);
+      }
+    const int k0 = t * kWideKeys;
+    if (a.zero_scale || k0 + kWideKeys > Tk) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          s[kb][j] = k0 + 32 * kb + 8 * (j >> 2) + 4 * hf + (j & 3) < Tk ? (a.zero_scale ? 0.f : s[kb][j]) : kNegInf;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[kb][j]);
+    mx = half_max(mx);
+    const float mc = mx * c2;
+    if (wave_any(mc > m_run)) {   // raised in whole steps, as in rows_body
+      const float m_new = m_run == kNegInf ? mc : raise_max(m_run, mc);
+      const float alpha = m_run == kNegInf ? 0.f : exp2_fast(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) oacc[nb] *= alpha;
+      m_run = m_new;
+    }
+    const float mneg = m_run == kNegInf ? 0.f : -m_run;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {   // 16 keys
+      float p[8], q[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = exp2_fast(fmaf(s[c >> 1][8 * (c & 1) + e], c2, mneg));
+        q[e] = p[e] - (float)(T)p[e];
+      }
+      l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      const V8 hi = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+      const V8 lo = pack8<T>(q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7]);
+      const int vrow = 16 * c + tr_row;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int col = nb * 32 + tr_col;
+        const char* x = vt + vrow * ROWB + (((col >> 3) ^ swz_v<D>(vrow)) * 16) + (col & 7) * 2;
+        const V8 va = cat_tr<T>(lds_read_tr(x), lds_read_tr(x + 8 * ROWB));
+        oacc[nb] = mfma32(va, hi, oacc[nb]);
+        oacc[nb] = mfma32(va, lo, oacc[nb]);
+      }
+    }
+    if (t + 1 < t_hi) {
+      store((t + 1 - t_lo) & 1);   // (read last in tile t - 1, before the barrier that ended it)
+      __syncthreads();
+    }
+  }
+  const float l_tot = half_sum(l_run);
+  if (row >= R) return;
+  const int64_t pr = ((int64_t)sp * a.B * a.Hq + (int64_t)b * a.Hq + h) * a.Tq + tq;
+  if (hf == 0) *(f32x4*)(a.part_ml + 4 * pr) = f32x4{m_run, l_tot, kNegInf, 0.f};
+  if (m_run == kNegInf) return;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int gi = 0; gi < 4; ++gi) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = oacc[nb][gi * 4 + e];
+      *(f32x4*)(a.part_o + pr * D + nb * 32 + gi * 8 + hf * 4) = x;
+    }
+}
+
 template <typename T, int D, bool MASK, bool SCORE, bool KW>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void prefix_rows_kernel(const PrefixArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[rows_lds<D, MASK>()];
   __shared__ float sml[kWaves][3][32];       // running maximum, sum, largest raw logit per wave and row
   // the prefix ranges first: the longest ones
+  if constexpr (D <= 128) {
+    static_assert(4 * kWideKeys * 2 * D <= rows_lds<D, MASK>(), "two buffers of K and V");
+    if (a.wide && (int)blockIdx.x < a.np) {
+      wide_body<T, D>(a, xcd_remap(blockIdx.x, a.np), smem);
+      return;
+    }
+  }
   if ((int)blockIdx.x < a.np) rows_body<T, D, false, false, false, false>(a, xcd_remap(blockIdx.x, a.np), smem, sml);
   else rows_body<T, D, true, MASK, SCORE, KW>(a, xcd_remap(blockIdx.x - a.np, a.no), smem, sml);
 }

@@ -6,7 +6,9 @@
 // below 2^32 (a product in fp32 has lost 0.06 rad at position 10^6).  Cosines and sines are made
 // once per token, into LDS, for all of its heads.
 //
-// What bounds it: reading and writing queries and keys once.
+// What bounds it: reading and writing queries and keys once, 8192 tokens of 40 heads of 128 at 5.4
+// TB/s.  The outputs are stored past the caches (a launch writes more than the L2s hold, and
+// lines kept for them push out the inputs: 7996 tokens of 32 heads of 80 24.6 -> 17.0 us).
 #include "fa_cache.h"
 #include "fa_common.h"
 
@@ -15,10 +17,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;   // head dims up to 256
-constexpr int kTok = 4;          // tokens of a workgroup
 
-// V columns per piece: 8 (16 bytes) or 1.
-template <typename T, int V, bool ADJ>
+// V columns per piece: 8 (16 bytes) or 1; kTok tokens per workgroup.
+template <typename T, int V, bool ADJ, int kTok>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   __shared__ float cs[2][kTok][kMaxPairs];   // cosines, sines
   const int64_t tok0 = (int64_t)blockIdx.x * kTok, ntok = (int64_t)a.B * a.T;
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   const int c0 = turned ? pc * V : 2 * a.R2 + (pc - NR) * V;
   const int c1 = ADJ ? (V == 1 && turned ? c0 ^ 1 : c0) : (turned ? c0 + a.R2 : c0);
   // kFly pieces at a time: their loads go out together
-  constexpr int kFly = 4;
+  constexpr int kFly = 2;
   while (tk < nt) {
     TV x0[kFly], x1[kFly];
     T* dst[kFly];
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
     for (int u = 0; u < kFly; ++u) {
       if (at[u] >= nt) continue;
       if (!turned) {
-        *(TV*)(dst[u] + c0) = x0[u];
+        __builtin_nontemporal_store(x0[u], (TV*)(dst[u] + c0));
       } else if constexpr (ADJ && V == 1) {
         const float co = cs[0][at[u]][c0 >> 1], si = cs[1][at[u]][c0 >> 1];
         const float x = (float)x0[u][0], y = (float)x1[u][0];
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
           y[e] = (T)fmaf(p, co, -(q * si));
           y[e + 1] = (T)fmaf(q, co, p * si);
         }
-        *(TV*)(dst[u] + c0) = y;
+        __builtin_nontemporal_store(y, (TV*)(dst[u] + c0));
       } else {
         TV y0, y1;
 #pragma unroll
@@ -117,20 +118,28 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
           y0[e] = (T)fmaf(p, co, -(q * si));
           y1[e] = (T)fmaf(q, co, p * si);
         }
-        *(TV*)(dst[u] + c0) = y0;
-        *(TV*)(dst[u] + c1) = y1;
+        __builtin_nontemporal_store(y0, (TV*)(dst[u] + c0));
+        __builtin_nontemporal_store(y1, (TV*)(dst[u] + c1));
       }
     }
   }
 }
 
-template <typename T> hipError_t launch_t(const RotaryArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.B * a.T + kTok - 1) / kTok)), block(kThreads);
-  if (a.vec && a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, 8, true>), grid, block, 0, s, a);
-  else if (a.vec) hipLaunchKernelGGL((rotary_kernel<T, 8, false>), grid, block, 0, s, a);
-  else if (a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, 1, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, block, 0, s, a);
+template <typename T, int TOK> hipError_t launch_n(const RotaryArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)a.B * a.T + TOK - 1) / TOK)), block(kThreads);
+  if (a.vec && a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, 8, true, TOK>), grid, block, 0, s, a);
+  else if (a.vec) hipLaunchKernelGGL((rotary_kernel<T, 8, false, TOK>), grid, block, 0, s, a);
+  else if (a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, 1, true, TOK>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, 1, false, TOK>), grid, block, 0, s, a);
   return hipGetLastError();
+}
+
+// One token per workgroup where the grid is small or a token is 8 KB or more, else two: 32 tokens of
+// 40 heads of 128 3.7 us (two 4.6), 8192 of them 30.9 (32.4); 7996 tokens of 32 heads of 80, 5 KB
+// each, 20.4 (17.0).
+template <typename T> hipError_t launch_t(const RotaryArgs& a, hipStream_t s) {
+  const bool one = (int64_t)a.B * a.T <= 1024 || (int64_t)(a.Hq + a.Hk) * a.D * 2 >= 8192;
+  return one ? launch_n<T, 1>(a, s) : launch_n<T, 2>(a, s);
 }
 
 }  // namespace

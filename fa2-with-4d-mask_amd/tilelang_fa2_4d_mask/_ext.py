@@ -116,7 +116,8 @@ class FaPrefixParams(ctypes.Structure):
 
 
 class FaPrefixPlan(ctypes.Structure):
-    _fields_ = _fields(("few_rows prefix_split own_split needs_mask_ws", _i32), ("workspace_bytes", _i64))
+    _fields_ = _fields(("few_rows prefix_split own_split needs_mask_ws", _i32), ("workspace_bytes", _i64),
+                       ("wide_rows reserved", _i32))
 
 
 class FaKeyWeightsParams(ctypes.Structure):

@@ -165,16 +165,15 @@ def _empty_attention(q, bhsd: bool):
 
 
 def _attend(q, k, v, pk, pv, lengths, mask, score, kw, scale, causal, weights, residual, bhsd):
-    """O, LSE, O's rounding residual (or empty), key weights (or empty)."""
+    """O, LSE, O's rounding residual (or None), key weights (or None)."""
     B, Tq, Tp, Tk, Hq, Hk, D = _sizes(q, k, pk, bhsd)
     if Tp == 0:
         pk = pv = None
-    if B * Tq * Hq == 0 or Tp + Tk == 0 or D == 0:
+    if B * Tq * Hq * D == 0 or Tp + Tk == 0:
         o, lse = _empty_attention(q, bhsd)
-        kw_out = q.new_empty((0,), dtype=torch.float32)
         if weights:
-            kw_out = q.new_zeros((B, Hk, Tk), dtype=torch.float32) if kw is None else kw.clone()
-        return o, lse, q.new_empty((0,)), kw_out
+            return o, lse, None, q.new_zeros((B, Hk, Tk), dtype=torch.float32) if kw is None else kw.clone()
+        return o, lse, None, None
     return _timed("fa_prefix_fwd", _host().attend, q, k, v, pk, pv, lengths, mask, score, kw, scale, causal, weights,
                   residual, bhsd)
 
@@ -185,7 +184,8 @@ def prefix_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pk: Optional[t
                scale: float, causal: bool, atomic: bool, residual: bool,
                bhsd: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """O (layout of q), LSE [B, Hq, Tq] fp32, O's rounding residual (with ``residual``, else empty)."""
-    return _attend(q, k, v, pk, pv, lengths, mask, score, None, scale, causal, False, residual, bhsd)[:3]
+    o, lse, lo, _ = _attend(q, k, v, pk, pv, lengths, mask, score, None, scale, causal, False, residual, bhsd)
+    return o, lse, q.new_empty((0,)) if lo is None else lo
 
 
 def _like_output(q, bhsd: bool):

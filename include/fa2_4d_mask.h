@@ -318,13 +318,15 @@ typedef struct FaPrefixParams {
 } FaPrefixParams;
 
 typedef struct FaPrefixPlan {
-  int32_t few_rows;              /* 1: rows packed in blocks of 32, the prefix read once for the batch; kw_out and
+  int32_t few_rows;              /* 1: rows packed in blocks, the prefix read once for the batch; kw_out and
                                     lengths are taken.  0: the 256-row blocks of fa_fwd for both key sets;
                                     neither is (lengths as part of the mask, fa_key_weights for the weights) */
   int32_t prefix_split;          /* key ranges of the prefix */
   int32_t own_split;             /* key ranges of the own keys */
   int32_t needs_mask_ws;         /* 1: a mask needs its prepared workspace (mask_ws) */
   int64_t workspace_bytes;       /* size of FaPrefixParams.workspace */
+  int32_t wide_rows;             /* few_rows: 1 if the prefix's blocks are of 128 rows, 0 if of 32 */
+  int32_t reserved;
 } FaPrefixPlan;
 
 /* From sizes, head dims, dtype, is_causal, and whether mask / score / kw_out are non-NULL. */

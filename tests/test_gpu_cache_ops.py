@@ -108,6 +108,11 @@ FORWARD = [
     (3, 4, 1, 256, 1, 700, 300, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),
     (2, 4, 2, 256, 40, 65, 100, FP, "ragged", "bernoulli", "normal", True, None, "bhsd", "contiguous"),
     (2, 2, 1, 200, 5, 33, 31, BF, None, None, None, True, None, "bshd", "contiguous"),
+    # enough rows and prefix for the blocks of 128 rows (a last block of few rows, a last tile of few keys)
+    (40, 32, 16, 64, 1, 4099, 33, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),
+    (17, 32, 8, 128, 2, 4097, 20, FP, None, "rows", None, False, -0.09, "bshd", "contiguous"),
+    (23, 48, 16, 96, 1, 4160, 0, BF, None, None, None, False, None, "bhsd", "slice"),
+    (65, 16, 16, 80, 1, 4095, 40, BF, "ragged", None, "normal", False, 0.0, "bhsd", "contiguous"),
     # more rows than a block of 32 per head: the 256-row blocks
     (2, 4, 2, 128, 33, 65, 100, BF, None, None, None, True, None, "bhsd", "token_major"),
     (2, 4, 2, 64, 257, 300, 257, FP, None, None, None, True, None, "bhsd", "contiguous"),
@@ -121,6 +126,25 @@ FORWARD = [
 
 def _id(c):
     return f"B{c[0]}H{c[1]}-{c[2]}D{c[3]}T{c[4]}-{c[5]}+{c[6]}{c[8] or ''}{c[9] or ''}{c[10] or ''}{'c' if c[11] else ''}"
+
+
+def test_the_prefix_plan_of_the_cases(cuda):
+    """Each way to run the prefix is among the cases: in blocks of 32 rows, of 128, of 256."""
+    import ctypes
+
+    from tilelang_fa2_4d_mask import _ext
+
+    ways = set()
+    for B, Hq, Hk, D, Tq, Tp, Tk, *_ in FORWARD:
+        p, plan = _ext.FaPrefixParams(), _ext.FaPrefixPlan()
+        p.batch, p.seqlen_q, p.seqlen_p, p.seqlen_k, p.heads_q, p.heads_k = B, Tq, Tp, Tk, Hq, Hk
+        p.head_dim = 64 if D <= 64 else (128 if D <= 128 else 256)
+        p.scale = 1.0
+        _ext.check(_ext.load_library().fa_prefix_plan(ctypes.byref(p), ctypes.byref(plan)), "fa_prefix_plan")
+        ways.add((plan.few_rows, plan.wide_rows, p.head_dim, plan.prefix_split > 1, plan.own_split > 1))
+    assert {(few, wide, d) for few, wide, d in ((1, 0, 64), (1, 0, 128), (1, 0, 256), (1, 1, 64), (1, 1, 128), (0, 0, 64),
+                                                (0, 0, 128))} <= {w[:3] for w in ways}
+    assert {(1, True, False), (1, False, True), (0, True, False)} <= {(w[0], w[3], w[4]) for w in ways}
 
 
 @pytest.mark.parametrize("case", FORWARD, ids=_id)
@@ -290,6 +314,7 @@ WEIGHTS = [
     (2, 4, 2, 64, 6, 0, 300, BF, "ragged", None, "lowest", False, None, "bhsd", "contiguous"),
     (2, 4, 2, 64, 6, 9, 100, BF, None, "late", "-inf", False, None, "bhsd", "contiguous"),
     (3, 4, 1, 256, 3, 20, 300, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),
+    (20, 32, 8, 128, 1, 8200, 77, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),   # (128-row blocks)
     # many rows: the sums in a pass of their own
     (2, 4, 2, 128, 40, 0, 40, BF, None, None, None, True, None, "bhsd", "token_major"),
     (2, 8, 2, 64, 257, 65, 300, FP, "ragged", None, None, False, None, "bshd", "contiguous"),
