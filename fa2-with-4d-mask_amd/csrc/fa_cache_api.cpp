@@ -66,11 +66,16 @@ void scales(float scale, float* scale_log2, float* qsign, int* zero) {
 
 // ---- shared prefix ------------------------------------------------------------------------
 
-// Rows per sequence up to which they are packed in blocks of 32 (fa_prefix.hip), each reading its
-// key set once; beyond, the 256-row blocks of fa_fwd.hip run over both key sets in turn, every
-// range leaving its partial result for one combine.  (Head dim 256: always packed; its own
-// forward leaves no partial results.)
-constexpr int kFewRows = 32;
+// Few rows per sequence: packed in blocks (fa_prefix.hip), the prefix read once for the batch.
+// Beyond, the 256-row blocks of fa_fwd.hip run over both key sets in turn, every range leaving its
+// partial result for one combine.  (Head dim 256: always packed; its own forward leaves no
+// partial results.)  In us, packed / not (bf16): 8 sequences behind 2000 shared keys, Hq 16, D 128, Tq
+// 48 33 / 69, 100 48 / 71, 200 70 / 84; one sequence behind 16000, Hq 32, Tq 48
+// 43 / 101, 100 70 / 108, 200 137 / 125; own keys alone, B16 Tk Tq + 500 Hq16 D64, Tq 48 21 / 28, 100
+// 34 / 30, 200 58 / 37.
+bool few_rows(const FaPrefixParams* p) {
+  return p->head_dim > 128 || p->seqlen_q <= (p->seqlen_p >= p->seqlen_k ? 128 : 64);
+}
 
 struct PrefixPlan {
   bool few, wide;
@@ -84,7 +89,7 @@ PrefixPlan prefix_plan(const FaPrefixParams* p) {
   const int G = p->heads_q / p->heads_k, kt = fa::prefix_tile_keys();
   const int64_t TG = (int64_t)G * p->seqlen_q;
   f.rows = (int64_t)p->batch * p->heads_q * p->seqlen_q;
-  f.few = p->seqlen_q <= kFewRows || p->head_dim > 128;
+  f.few = few_rows(p);
   if (!f.few) {
     auto ranges = [&](int64_t Tk, bool causal) -> int {
       if (Tk == 0) return 0;
@@ -94,7 +99,8 @@ PrefixPlan prefix_plan(const FaPrefixParams* p) {
     };
     f.nsp = ranges(p->seqlen_p, false);
     f.nso = ranges(p->seqlen_k, p->is_causal != 0);
-    f.bytes = f.rows * (f.nsp + f.nso) * (p->head_dim + 2) * (int64_t)sizeof(float);
+    // (a single range writes O itself)
+    f.bytes = f.nsp + f.nso == 1 ? 0 : f.rows * (f.nsp + f.nso) * (p->head_dim + 2) * (int64_t)sizeof(float);
     return f;
   }
   // The prefix in blocks of 128 rows sharing its 64-key tiles, where those give every CU four tiles;
@@ -146,7 +152,7 @@ int check_prefix(const FaPrefixParams* p) {
 }
 
 bool kw_fits(const FaPrefixParams* p) {
-  return p->seqlen_q <= kFewRows && (int64_t)(p->heads_q / p->heads_k) * p->seqlen_q <= fa::kPrefixKwRows;
+  return few_rows(p) && (int64_t)(p->heads_q / p->heads_k) * p->seqlen_q <= fa::kPrefixKwRows;
 }
 
 // Both key sets through the 256-row forward, then one combine of all ranges.
@@ -162,8 +168,8 @@ int prefix_many(const FaPrefixParams* p, const PrefixPlan& f) {
   a.nqt = (int)ceil_div(p->seqlen_q, fa::kFwdRows);   // (the precise forms' blocks)
   a.fine = 1;
   const int64_t rows = f.rows, ns = f.nsp + f.nso;
-  float* part_o = (float*)p->workspace;
-  float* part_ml = part_o + rows * ns * p->head_dim;
+  float* part_o = ns > 1 ? (float*)p->workspace : nullptr;
+  float* part_ml = ns > 1 ? part_o + rows * ns * p->head_dim : nullptr;
   const hipStream_t s = (hipStream_t)p->stream;
   int st;
   if (f.nsp) {
@@ -188,9 +194,14 @@ int prefix_many(const FaPrefixParams* p, const PrefixPlan& f) {
       x.mws = (const char*)p->mask_ws;
       x.ml = fa::mask_layout(p->batch, p->heads_q, p->seqlen_q, p->seqlen_k, p->mask_stride_b == 0, p->mask_stride_h == 0);
     }
-    x.ns = f.nso; x.part_o = part_o + f.nsp * rows * p->head_dim; x.part_ml = part_ml + 2 * f.nsp * rows;
+    x.ns = f.nso;
+    if (ns > 1) {
+      x.part_o = part_o + f.nsp * rows * p->head_dim;
+      x.part_ml = part_ml + 2 * f.nsp * rows;
+    }
     if ((st = launch_status(fa::launch_fwd(x, p->head_dim, p->dtype, causal, s), "fa_prefix_fwd own"))) return st;
   }
+  if (ns == 1) return FA_OK;
   a.ns = (int)ns; a.part_o = part_o; a.part_ml = part_ml;
   return launch_status(fa::launch_fwd_combine(a, p->head_dim, p->dtype, s), "fa_prefix_fwd combine");
 }
@@ -239,10 +250,10 @@ int fa_prefix_fwd(const FaPrefixParams* p) {
     if (own && p->score && (31 * p->score_stride_q + (int64_t)p->seqlen_k + 64) * 4 >= (1LL << 32))
       return fail(FA_ERR_STRIDE, "score query stride %lld: 32 score rows must span less than 4 GiB", (long long)p->score_stride_q);
   }
-  if (!p->workspace || p->workspace_bytes < f.bytes)
+  if (f.bytes && (!p->workspace || p->workspace_bytes < f.bytes))
     return fail(FA_ERR_WORKSPACE, "workspace of %lld bytes needed, %lld given", (long long)f.bytes,
                 (long long)(p->workspace ? p->workspace_bytes : 0));
-  if (!aligned16(p->workspace)) return fail(FA_ERR_STRIDE, "workspace must be 16-byte aligned");
+  if (f.bytes && !aligned16(p->workspace)) return fail(FA_ERR_STRIDE, "workspace must be 16-byte aligned");
   if (!f.few) return prefix_many(p, f);
 
   fa::PrefixArgs a{};

@@ -114,8 +114,9 @@ __device__ __forceinline__ void lds_barrier() {
 // FULL: all D columns of the operands exist; otherwise Dv do (a run-time value in the
 // prologue and the epilogue, 0.2-1.5 us of a launch: not where a short problem in one
 // range would notice).
-// FINE (a split without a mask or score): P enters O in two parts all the same, for a softmax
-// that goes on over another key set, whose backward takes Delta from an O that must match it.
+// FINE (without a mask or score): P enters O in two parts all the same, for a softmax that goes
+// on over another key set, whose backward takes Delta from an O that must match it, and for
+// key weights.
 template <typename T, int D, bool CAUSAL, bool MASK, bool SCORE, bool SPLIT, bool FULL, bool FINE = false>
 __global__ __launch_bounds__(fwd_waves(D, CAUSAL, MASK || FINE, SCORE) * 64, fwd_waves(D, CAUSAL, MASK || FINE, SCORE) == 4 ? 3 : 1) void fwd_kernel(const FwdArgs a) {
   const int Dv = FULL ? D : a.Dv;
@@ -841,12 +842,13 @@ __global__ __launch_bounds__(fwd_waves(D, CAUSAL, MASK || FINE, SCORE) * 64, fwd
 #pragma unroll
         for (int gi = 0; gi < 4; ++gi) {
           const int d = nb * 32 + gi * 8 + hf * 4;
+          // (less what was stored, not a rounding of o anew: o's product may enter its rounding
+          // unrounded there, and then falls on the other side of a tie now and then)
+          T st[4];
+          __builtin_memcpy(st, os + l32 * OS + d, 8);
           float r[4];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const float o = oacc[nb][gi * 4 + t] * inv;
-            r[t] = o - (float)(T)o;
-          }
+          for (int t = 0; t < 4; ++t) r[t] = oacc[nb][gi * 4 + t] * inv - (float)st[t];
           lds_write8(os + l32 * OS + d, pack4<T>(r[0], r[1], r[2], r[3]));
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -882,7 +884,8 @@ template <typename T, int D, bool CAUSAL>
 hipError_t launch_fwd_c(const FwdArgs& a, hipStream_t s) {
   if (a.fine && !a.mask && !a.score) {
     const dim3 grid((unsigned)(a.B * a.Hq * a.nqt * a.ns)), block(fwd_waves(D, CAUSAL, true, false) * 64);
-    hipLaunchKernelGGL((fwd_kernel<T, D, CAUSAL, false, false, true, false, true>), grid, block, 0, s, a);
+    if (a.part_o) hipLaunchKernelGGL((fwd_kernel<T, D, CAUSAL, false, false, true, false, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((fwd_kernel<T, D, CAUSAL, false, false, false, false, true>), grid, block, 0, s, a);
     return hipGetLastError();
   }
   if (a.part_o) return launch_fwd_t<T, D, CAUSAL, true, false>(a, s);   // (also a single range's partial result)

@@ -16,25 +16,27 @@
 //                        their largest raw logit and their sum anew; others leave at once.
 #include "fa_cache.h"
 #include "fa_common.h"
+#include "fa_pipe.h"
 
 namespace fa {
 namespace {
 
+using pipe::IC;
+
 constexpr int kWaves = 4;
-template <int D> constexpr int frags() { return D == 256 ? 1 : 2; }   // 32-key fragments per wave
+template <int D> constexpr int frags() { return D == 256 ? 1 : 2; }       // 32-key fragments per wave
+template <int D> constexpr int tile_rows() { return D == 256 ? 32 : 64; }
+// Chunk swizzle of the row tiles: 16 rows' reads of one chunk hit 64 distinct banks.
+template <int D> __device__ __forceinline__ int swz(int r) { return pipe::swz_q<D == 64 ? 64 : 128>(r); }
 
 __device__ __forceinline__ int own_length(const KeyWArgs& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
 }
 
-// The row lane l32 of a 32-row tile reads, of a kv-head's group: r = g Tq + tq.
+// A row of a kv-head's group, r = g Tq + tq.
 struct Row {
   int g, tq;
 };
-__device__ __forceinline__ Row row_of(const KeyWArgs& a, int r) {
-  const int g = r / a.Tq;
-  return {g, r - g * a.Tq};
-}
 
 template <typename T, int DS> __device__ __forceinline__ void load_q(const KeyWArgs& a, u32x4 (&x)[DS], int b, int h, int tq, int hf) {
   load_row(x, (const T*)a.q + b * a.qsb + h * a.qsh + (int64_t)tq * a.qst + hf * 8, a.Dv);
@@ -85,54 +87,99 @@ __device__ __forceinline__ f32x16 scores(const float* srow, int k0, int hf, int 
 template <typename T, int D, bool MASK, bool SCORE>
 __global__ __launch_bounds__(kWaves * 64, 2) void key_weights_kernel(const KeyWArgs a) {
   using V8 = typename Vec8<T>::type;
-  constexpr int DS = D / 16, NF = frags<D>();
-  const int W = xcd_remap(blockIdx.x, a.B * a.Hk * a.ns * a.nkb);
-  const int kb = W % a.nkb, W1 = W / a.nkb;   // (causal: the first key blocks have the most rows)
-  const int sp = W1 % a.ns, bk = W1 / a.ns;
+  constexpr int DS = D / 16, NF = frags<D>(), CH = D / 8, RT = tile_rows<D>();
+  constexpr int NU = RT * CH / (kWaves * 64);   // 16-byte chunks of a tile per thread
+  __shared__ __align__(16) char tiles[2][RT * D * 2];
+  __shared__ float lses[2][RT];
+  // causal: the first key blocks have the most rows, so all of them start first
+  const int n_per = a.B * a.Hk * a.ns, kb = blockIdx.x / n_per, W = blockIdx.x - kb * n_per;
+  const int sp = W % a.ns, bk = W / a.ns;
   const int b = bk / a.Hk, kvh = bk - b * a.Hk;
   const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = own_length(a, b);
-  const int k0 = (kb * kWaves + wave) * NF * 32;   // this wave's first key
-  const int R = a.G * a.Tq, nt = (R + 31) / 32;
+  const int kb0 = kb * kWaves * NF * 32, k0 = kb0 + wave * NF * 32;   // the workgroup's first key, this wave's
+  const int R = a.G * a.Tq, nt = (R + RT - 1) / RT;
   const float c2 = a.scale_log2;
   const uint32_t neg = a.qsign < 0.f ? 0x80008000u : 0u;
 
   f32x16 acc[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) acc[f] = f32x16{};
-  if (k0 < n) {
+  if (kb0 < n) {
     const T* kp = (const T*)a.k + b * a.ksb + kvh * a.ksh;
     V8 kf[NF][DS];
 #pragma unroll
     for (int f = 0; f < NF; ++f) load_keys<T, DS>(a, kp, k0 + 32 * f, n, l32, hf, kf[f]);
-    // the next tile some row of which sees key k0
-    auto next = [&](int t) __attribute__((always_inline)) -> int {
+    // Tile t starts at row (g, tq) of the group, and the tile ns behind it dg heads and dt rows on.
+    struct Tile {
+      int t, g, tq;
+    };
+    const int dg = RT * a.ns / a.Tq, dt = RT * a.ns - dg * a.Tq;
+    auto behind = [&](Tile x) __attribute__((always_inline)) -> Tile {
+      x.t += a.ns;
+      x.g += dg;
+      x.tq += dt;
+      if (x.tq >= a.Tq) {
+        x.tq -= a.Tq;
+        ++x.g;
+      }
+      return x;
+    };
+    // causal: the first tile from x on some row of which sees key kb0 (a tile of one head's last
+    // rows and the next one's first: always)
+    auto seen = [&](Tile x) __attribute__((always_inline)) -> Tile {
       if (a.causal)
-        for (; t < nt; t += a.ns) {
-          const Row lo = row_of(a, t * 32), hi = row_of(a, min(t * 32 + 31, R - 1));
-          if (lo.g != hi.g || hi.tq >= k0) break;
+        while (x.t < nt && x.tq + RT <= a.Tq && x.tq + RT <= kb0) x = behind(x);
+      return x;
+    };
+    auto row_in = [&](const Tile& x, int i) __attribute__((always_inline)) -> Row {   // row i (past R: the last)
+      if (x.t * RT + i >= R) return {a.G - 1, a.Tq - 1};
+      int g = x.g, tq = x.tq + i;
+      if (a.Tq >= RT) {
+        if (tq >= a.Tq) {
+          tq -= a.Tq;
+          ++g;
         }
-      return t;
+      } else {
+        const int y = tq / a.Tq;
+        g += y;
+        tq -= y * a.Tq;
+      }
+      return {g, tq};
     };
-    u32x4 x[DS];
+    // A tile's rows and LSEs, loaded while the one before is worked on.
+    const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    constexpr int RS = kWaves * 64 / CH;   // rows between a thread's chunks
+    u32x4 x[NU];
     float e = 0.f;
-    auto load_tile = [&](int t) __attribute__((always_inline)) {
-      const int r = t * 32 + l32;
-      const Row q = row_of(a, min(r, R - 1));
-      load_q<T, DS>(a, x, b, kvh * a.G + q.g, q.tq, hf);
-      // rows past R: +inf, as a row without a kept key
-      e = r < R ? a.lse[((int64_t)b * a.Hq + kvh * a.G + q.g) * a.Tq + q.tq] : kPosInf;
+    auto load_tile = [&](const Tile& t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const Row q = row_in(t, r0 + u * RS);
+        x[u] = gload16((const T*)a.q + b * a.qsb + (kvh * a.G + q.g) * a.qsh + (int64_t)q.tq * a.qst + (8 * c < a.Dv ? 8 * c : 0));
+      }
+      if (threadIdx.x < RT) {
+        const Row q = row_in(t, threadIdx.x);
+        // rows past R: +inf, as a row without a kept key
+        e = t.t * RT + (int)threadIdx.x < R ? a.lse[((int64_t)b * a.Hq + kvh * a.G + q.g) * a.Tq + q.tq] : kPosInf;
+      }
     };
-    int t = next(sp);
-    if (t < nt) load_tile(t);
-    while (t < nt) {
+    auto keep_tile = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        lds_write16(tiles[buf] + (r0 + u * RS) * 2 * D + ((c ^ swz<D>(r0 + u * RS)) * 16),
+                    zero_unless(8 * c < a.Dv, x[u] ^ neg));
+      if (threadIdx.x < RT) lses[buf][threadIdx.x] = e;
+    };
+    // probabilities of 32 rows from LDS (this lane's: row q) added to the keys' sums; EDGE: some are
+    // dropped
+    auto add = [&](auto EDGEc, const char* rows, const Row& q, float lse) __attribute__((always_inline)) {
+      const int h = kvh * a.G + q.g;
       V8 qf[DS];
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec8<T>(only_cols(x[ds], ds, a.Dv, neg));
-      const Row q = row_of(a, min(t * 32 + l32, R - 1));
-      const int h = kvh * a.G + q.g;
-      float sub = 0.f, lse = e, mul = 1.f;
+      for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec8<T>(lds_read16(rows + l32 * 2 * D + ((2 * ds + hf) ^ swz<D>(l32)) * 16));
+      float sub = 0.f, mul = 1.f;
       if constexpr (SCORE) {
         if (far_max(lse) && lse != kPosInf) {
           const float* ml = a.far_ml + 2 * (((int64_t)b * a.Hq + h) * a.Tq + q.tq);
@@ -141,32 +188,69 @@ __global__ __launch_bounds__(kWaves * 64, 2) void key_weights_kernel(const KeyWA
           mul = 1.0f / ml[1];
         }
       }
-      const int t_nx = next(t + a.ns);
-      if (t_nx < nt) load_tile(t_nx);
-      const int lim = a.causal ? min(n, q.tq + 1) : n;
-      const bool edge = MASK || a.zero_scale || a.causal || k0 + 32 * NF > n;
+      // (with a mask or score a fragment at a time: their bits and rows need the registers)
+      constexpr int NS = MASK || SCORE ? 1 : NF;
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const int kk = k0 + 32 * f;
-        f32x16 s = f32x16{};
-        if constexpr (SCORE) s = scores(a.score + b * a.ssb + h * a.ssh + (int64_t)q.tq * a.ssq, kk, hf, n, a.qsign);
+      for (int f0 = 0; f0 < NF; f0 += NS) {
+        f32x16 s[NS];
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) s = mfma32(kf[f][ds], qf[ds], s);
-        uint32_t w = ~0u;
-        if (edge) {
-          w = in_row(lim, kk, hf);
-          if constexpr (MASK) w &= mask_bits(a, a.mask + b * a.msb + h * a.msh + (int64_t)q.tq * a.msq, kk, hf, n);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            s[j] = (w >> (8 * (j >> 2) + (j & 3))) & 1u ? (a.zero_scale ? 0.f : s[j]) : kNegInf;
+        for (int f = 0; f < NS; ++f) {
+          s[f] = f32x16{};
+          if constexpr (SCORE)
+            s[f] = scores(a.score + b * a.ssb + h * a.ssh + (int64_t)q.tq * a.ssq, k0 + 32 * (f0 + f), hf, n, a.qsign);
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if constexpr (SCORE) acc[f][j] += exp2_fast(fmaf(s[j] - sub, c2, -lse)) * mul;
-          else acc[f][j] += exp2_fast(fmaf(s[j], c2, -lse));
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+          for (int f = 0; f < NS; ++f) s[f] = mfma32(kf[f0 + f][ds], qf[ds], s[f]);
+        if constexpr (decltype(EDGEc)::value) {
+          const int lim = a.causal ? min(n, q.tq + 1) : n;
+#pragma unroll
+          for (int f = 0; f < NS; ++f) {
+            const int kk = k0 + 32 * (f0 + f);
+            uint32_t w = in_row(lim, kk, hf);
+            if constexpr (MASK) w &= mask_bits(a, a.mask + b * a.msb + h * a.msh + (int64_t)q.tq * a.msq, kk, hf, n);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              s[f][j] = (w >> (8 * (j >> 2) + (j & 3))) & 1u ? (a.zero_scale ? 0.f : s[f][j]) : kNegInf;
+          }
+        }
+#pragma unroll
+        for (int f = 0; f < NS; ++f)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if constexpr (SCORE) acc[f0 + f][j] += exp2_fast(fmaf(s[f][j] - sub, c2, -lse)) * mul;
+            else acc[f0 + f][j] += exp2_fast(fmaf(s[f][j], c2, -lse));
+          }
+        if constexpr (NS < NF) __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    const bool edge = MASK || a.zero_scale || k0 + 32 * NF > n;
+    const int g0 = RT * sp / a.Tq;
+    Tile t = seen(Tile{sp, g0, RT * sp - g0 * a.Tq});
+    if (t.t < nt) {
+      load_tile(t);
+      keep_tile(0);
+    }
+    __syncthreads();
+    for (int buf = 0; t.t < nt; buf ^= 1) {
+      const Tile now = t;
+      t = seen(behind(t));
+      if (t.t < nt) load_tile(t);
+      if (k0 < n) {
+#pragma unroll
+        for (int i = 0; i < RT; i += 32) {
+          const bool one = now.tq + i + 32 <= a.Tq;   // rows of one head
+          if (now.t * RT + i >= R || (a.causal && one && now.tq + i + 32 <= k0)) continue;
+          const char* rows = tiles[buf] + i * 2 * D;   // (32 rows on: the same swizzle)
+          const float lse = lses[buf][i + l32];
+          const Row q = row_in(now, i + l32);
+          if (edge || (a.causal && !(one && now.tq + i >= k0 + 32 * NF - 1))) add(IC<1>{}, rows, q, lse);
+          else add(IC<0>{}, rows, q, lse);
         }
       }
-      t = t_nx;
+      if (t.t < nt) keep_tile(buf ^ 1);   // (its last readers: before the barrier before this one)
+      __syncthreads();
     }
 #pragma unroll
     for (int f = 0; f < NF; ++f)

@@ -241,10 +241,10 @@ PREFIX_REFUSALS = [
     (dict(mask=FAKE, mask_stride_q=-1), 5), (dict(score=FAKE, score_stride_h=-4), 5),
     (dict(kw_in=FAKE, kw_out=FAKE, kw_stride_b=-1), 5), (dict(o_lo=FAKE, o_lo_stride_t=4), 5),
     (dict(workspace=None), 8), (dict(workspace_bytes=100), 8), (dict(workspace=FAKE + 8), 5),
-    (dict(seqlen_q=33, kw_out=FAKE), 2), (dict(seqlen_q=33, lengths=FAKE), 2),
+    (dict(seqlen_q=129, kw_out=FAKE), 2), (dict(seqlen_q=129, lengths=FAKE), 2),
     (dict(seqlen_q=20, kw_out=FAKE), 2),                       # 80 rows of a group: the weights in a pass of their own
-    (dict(seqlen_q=33, mask=FAKE), 8), (dict(seqlen_q=33, mask=FAKE, mask_ws=FAKE + 16), 5),
-    (dict(seqlen_q=33, score=FAKE, score_stride_q=1 << 26), 5),
+    (dict(seqlen_q=129, mask=FAKE), 8), (dict(seqlen_q=129, mask=FAKE, mask_ws=FAKE + 16), 5),
+    (dict(seqlen_q=129, score=FAKE, score_stride_q=1 << 26), 5),
 ]
 
 
@@ -270,7 +270,7 @@ def test_prefix_plans(lib):
     few, nsp, nso, _, n = of(kw_out=FAKE, seqlen_k=513)      # whole tiles of 32 keys
     assert n == rows * ((nsp + nso) * (128 + 4) + 544) * 4
     assert of(seqlen_p=0)[1] == 0 and of(seqlen_k=0)[2] == 0
-    assert of(seqlen_q=33)[0] == 0 and of(seqlen_q=33)[3] == 1
+    assert of(seqlen_q=129)[0] == 0 and of(seqlen_q=129)[3] == 1
     assert of(seqlen_q=20, kw_out=FAKE)[0] == 0 and of(seqlen_q=20)[0] == 1
     assert of(seqlen_q=4096, head_dim=256)[0] == 1           # head dim 256 is always packed
     assert lib.fa_prefix_plan(None, ctypes.byref(plan)) == 1

@@ -113,7 +113,7 @@ FORWARD = [
     (17, 32, 8, 128, 2, 4097, 20, FP, None, "rows", None, False, -0.09, "bshd", "contiguous"),
     (23, 48, 16, 96, 1, 4160, 0, BF, None, None, None, False, None, "bhsd", "slice"),
     (65, 16, 16, 80, 1, 4095, 40, BF, "ragged", None, "normal", False, 0.0, "bhsd", "contiguous"),
-    # more rows than a block of 32 per head: the 256-row blocks
+    # more rows per head, on both sides of what decides for the 256-row blocks
     (2, 4, 2, 128, 33, 65, 100, BF, None, None, None, True, None, "bhsd", "token_major"),
     (2, 4, 2, 64, 257, 300, 257, FP, None, None, None, True, None, "bhsd", "contiguous"),
     (3, 4, 2, 128, 300, 0, 300, BF, "ragged", None, None, True, None, "bhsd", "contiguous"),
@@ -121,6 +121,19 @@ FORWARD = [
     (2, 4, 2, 128, 65, 513, 200, BF, "ragged", "bernoulli", "normal", False, -0.1, "bshd", "contiguous"),
     (2, 4, 4, 64, 130, 40, 130, FP, None, None, "lowest", True, None, "bhsd", "contiguous"),
     (1, 8, 8, 40, 70, 10, 70, BF, None, "rows", None, False, 0.0, "bhsd", "contiguous"),
+    (2, 4, 2, 128, 64, 30, 100, BF, None, None, None, True, None, "bhsd", "contiguous"),
+    (2, 4, 2, 64, 128, 100, 100, FP, "ragged", None, None, False, None, "bshd", "contiguous"),
+    (2, 4, 2, 128, 133, 165, 140, BF, None, None, None, True, None, "bhsd", "token_major"),
+    (2, 4, 2, 96, 150, 1100, 0, BF, None, None, None, False, None, "bhsd", "slice"),
+    (2, 4, 2, 128, 129, 513, 200, BF, "ragged", "bernoulli", "normal", False, -0.1, "bshd", "contiguous"),
+    (1, 8, 8, 40, 170, 180, 170, BF, None, "rows", None, False, 0.0, "bhsd", "contiguous"),
+    (2, 4, 2, 64, 300, 77, 500, FP, "past", "late", None, True, None, "bhsd", "contiguous"),
+    # one range of one key set
+    (2, 4, 2, 64, 70, 0, 200, BF, "ragged", "bernoulli", None, True, None, "bhsd", "contiguous"),
+    (2, 4, 2, 128, 140, 0, 90, FP, None, None, "normal", False, None, "bshd", "slice"),
+    (2, 4, 2, 128, 140, 0, 90, FP, None, None, "lowest", True, None, "bhsd", "contiguous"),
+    (2, 16, 16, 96, 260, 0, 300, BF, "past", None, None, True, 0.0, "bhsd", "contiguous"),
+    (2, 4, 1, 64, 270, 90, 0, BF, None, None, None, False, -0.1, "bshd", "token_major"),
 ]
 
 
@@ -193,6 +206,9 @@ BACKWARD = [
     (2, 4, 2, 64, 20, 35, 0, BF, None, None, None, False, None, "bhsd", "contiguous"),
     (2, 16, 4, 128, 300, 700, 300, BF, None, None, None, True, None, "bhsd", "contiguous"),
     (1, 4, 2, 64, 40, 40, 40, BF, None, None, None, True, 0.0, "bhsd", "contiguous"),
+    (3, 4, 2, 64, 131, 133, 131, FP, "ragged", None, None, True, None, "bhsd", "contiguous"),
+    (2, 4, 2, 128, 140, 200, 150, BF, None, "rows", "normal", False, None, "bshd", "slice"),
+    (2, 4, 2, 64, 140, 0, 140, BF, None, None, None, True, None, "bhsd", "contiguous"),
 ]
 
 
@@ -325,6 +341,9 @@ WEIGHTS = [
     (1, 4, 4, 256, 50, 0, 300, BF, None, None, None, True, 0.0, "bhsd", "contiguous"),
     (1, 8, 1, 64, 1000, 0, 129, BF, None, None, None, False, None, "bhsd", "contiguous"),
     (2, 16, 1, 64, 5, 0, 129, FP, "ragged", None, "-inf", False, None, "bhsd", "contiguous"),
+    (2, 4, 2, 64, 140, 30, 200, FP, None, "late", "lowest", True, None, "bhsd", "contiguous"),
+    (2, 8, 2, 128, 131, 300, 299, BF, "ragged", None, None, True, None, "bshd", "contiguous"),
+    (1, 6, 2, 128, 700, 0, 520, BF, None, None, None, True, None, "bhsd", "token_major"),
 ]
 
 
@@ -371,6 +390,7 @@ EVICT = [
     (2, 2, 700, 128, 128, 128, BF, "bhsd", "ragged", "rand"),  # the most recent alone
     (2, 2, 600, 40, 100, 5, FP, "bhsd", None, "odd"),          # NaN, infinities, -0, negative, subnormal
     (1, 8, 9001, 256, 33, 1, BF, "bhsd", None, "close"),       # weights that differ in their last bits
+    (2, 2, 33001, 24, 20000, 100, BF, "bhsd", "ragged", "few"),   # more weights than the LDS holds
 ]
 
 
@@ -554,9 +574,9 @@ def _calls(cuda, seed=51, B=3, Tk=700):
     r = lambda *s: torch.randn(s, generator=g).to(BF).to(cuda)  # noqa: E731
     Hq, Hk, D, Tp = 8, 2, 128, 900
     q, k, v, pk, pv = r(B, Hq, 1, D), r(B, Hk, Tk, D), r(B, Hk, Tk, D), r(1, Hk, Tp, D), r(1, Hk, Tp, D)
-    q2, w = r(B, Hq, 70, D), torch.rand((B, Hk, Tk), generator=g).to(cuda)
+    q2, w = r(B, Hq, 140, D), torch.rand((B, Hk, Tk), generator=g).to(cuda)
     n = torch.tensor([Tk, 1, Tk // 2], dtype=torch.int32, device=cuda)[:B]
-    pos = torch.arange(70, device=cuda).expand(1, 1, 70).contiguous()
+    pos = torch.arange(140, device=cuda).expand(1, 1, 140).contiguous()
     freq = torch.logspace(0, -3, 64, device=cuda)
     return (q, k, v, pk, pv, q2, w, n, pos, freq), {
         "prefix": lambda: (api.tilelang_shared_prefix_attention(q, k, v, pk, pv, lengths=n),),
@@ -647,8 +667,8 @@ def test_compiled_training_step(cuda):
     _, k, v, pk, pv, q, _, n, pos, freq = inputs
 
     def step(q, k, v, pk, pv):
-        q, kr = api.tilelang_rotary_embedding(q, k[:, :, :70], pos, freq)
-        return api.tilelang_shared_prefix_attention(q, kr, v[:, :, :70], pk, pv, is_causal=True, use_atomic_backward=False)
+        q, kr = api.tilelang_rotary_embedding(q, k[:, :, :140], pos, freq)
+        return api.tilelang_shared_prefix_attention(q, kr, v[:, :, :140], pk, pv, is_causal=True, use_atomic_backward=False)
 
     leaves = [x.clone().requires_grad_(True) for x in (q, k, v, pk, pv)]
     out = step(*leaves)
@@ -666,7 +686,7 @@ def test_captured_training_step(cuda):
     on changed inputs."""
     inputs, _ = _calls(cuda, 91)
     _, k, v, pk, pv, q, _, _, pos, freq = inputs
-    static = [x.clone().requires_grad_(True) for x in (q, k[:, :, :70].contiguous(), v[:, :, :70].contiguous(), pk, pv)]
+    static = [x.clone().requires_grad_(True) for x in (q, k[:, :, :140].contiguous(), v[:, :, :140].contiguous(), pk, pv)]
     do = torch.randn_like(q)
 
     def step(leaves):
