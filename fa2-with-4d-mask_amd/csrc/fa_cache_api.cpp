@@ -397,9 +397,11 @@ int fa_evict(const FaEvictParams* p) {
   a.B = p->batch; a.Tk = p->seqlen_k; a.Hk = p->heads_k; a.D = p->head_dim; a.keep = p->keep; a.recent = p->recent;
   a.vec = p->head_dim % 8 == 0 && aligned16(p->k) && aligned16(p->v) && aligned16(p->k_out) && aligned16(p->v_out);
   for (int64_t s : st) a.vec = a.vec && s % 8 == 0;
-  // two workgroups per CU, each with 64 rows to copy at least
+  // A workgroup per CU, each with 64 rows to copy at least: two would make each other wait for the
+  // same selection (B1 Tk 16384 Hk8 D128 keep 4096: 16.4 us, with two 26.9; B16 Tk 3001 Hk4 D96 keep
+  // 1500: 19.7 and 25.5; half as many: 17.3 and 20.3).
   const int64_t heads = (int64_t)p->batch * p->heads_k;
-  a.nw = (int)std::max(ceil_div(p->keep, fa::kEvictShare), std::min(ceil_div(2 * fa::kCus, heads), ceil_div(p->keep, 64)));
+  a.nw = (int)std::max(ceil_div(p->keep, fa::kEvictShare), std::min<int64_t>(std::max<int64_t>(fa::kCus / heads, 1), ceil_div(p->keep, 64)));
   if (heads * a.nw >= (1 << 21)) return fail(FA_ERR_SHAPE, "problem too large for one launch");
   return launch_status(fa::launch_evict(a, (hipStream_t)p->stream), "fa_evict");
 }
