@@ -311,7 +311,8 @@ using Pair = std::tuple<Tensor, Tensor>;
 Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Tensor& freq, const std::vector<int64_t>& sections,
                 bool adjacent, bool inverse, bool bhsd) {
   check_operands(q_, k_, k_);
-  TORCH_CHECK(k_.size(bhsd ? 2 : 1) == q_.size(bhsd ? 2 : 1), "q and k do not fit together");
+  TORCH_CHECK(k_.size(bhsd ? 2 : 1) == q_.size(bhsd ? 2 : 1) && q_.size(bhsd ? 1 : 2) > 0 && k_.size(bhsd ? 1 : 2) > 0,
+              "q and k do not fit together");
   TORCH_CHECK(pos.dim() == 3 && (pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) && pos.device() == q_.device() &&
                   pos.size(0) == (int64_t)sections.size() && (pos.size(1) == 1 || pos.size(1) == q_.size(0)) &&
                   pos.size(2) == q_.size(bhsd ? 2 : 1),

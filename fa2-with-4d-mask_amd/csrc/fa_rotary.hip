@@ -40,7 +40,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
     const double lo = fma(f, kTurnLo, fma(f, kTurn, -turns));
     float s, c;
     if (fabs(turns) < 0x1p28) {
-      const uint64_t turn = (uint64_t)((turns - floor(turns)) * 0x1p64) + (uint64_t)(int64_t)rint(lo * 0x1p64);
+      const double part = turns - rint(turns);   // exact, in [-1/2, 1/2]
+      const uint64_t turn = (uint64_t)(int64_t)rint((part < 0.5 ? part : -0.5) * 0x1p64) + (uint64_t)(int64_t)rint(lo * 0x1p64);
       const int32_t top = (int32_t)((turn * (uint64_t)pos) >> 32);   // in [-1/2, 1/2) turns, times 2^32
       sincospif((float)top * 0x1p-31f, &s, &c);
     } else {

@@ -37,6 +37,16 @@ _NS = "tilelang_fa2_4d_mask"
 # ---- checks ------------------------------------------------------------------------
 
 
+def _sizes_of(query, key, value, layout: str):
+    """(batch, heads_q, heads_k, seqlen_q, seqlen_k, head_dim), checked."""
+    if key.dim() == 4 and 0 in (key.shape[1 if layout == "bhsd" else 2], key.shape[3]):
+        raise ValueError("key and value must have at least one head and one column")
+    B, Hq, Tq, Tk, D = _dims(query, key, value, layout)
+    if D > 256:
+        raise ValueError(f"head dimension {D} is not supported (up to 256)")
+    return B, Hq, key.shape[1 if layout == "bhsd" else 2], Tq, Tk, D
+
+
 def _check_types(first: str, x: torch.Tensor, **others) -> None:
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"TileLang attention expects fp16 or bf16 inputs, got {x.dtype}")
@@ -322,20 +332,20 @@ def tilelang_shared_prefix_attention(
 
     query [B, Hq, Tq, D], key / value [B, Hk, Tk, D]: the own keys, Tk may be 0;
     prefix_key / prefix_value [1, Hk, Tp, D] (``layout="bshd"``: heads and tokens
-    exchanged), fp16 / bf16, GQA/MQA as in :func:`tilelang_flash_attention`.
+    exchanged), fp16 / bf16, D up to 256, GQA/MQA as in :func:`tilelang_flash_attention`.
     Every row sees the whole prefix; the following concern the own keys:
     lengths: int32 / int64 [B], the first ``lengths[b]`` keys exist (values are clamped
     to [0, Tk]; memory past them may hold anything).  mask: bool [B|1, Hq|1, Tq, Tk], True
     keeps.  score: float [B|1, Hq|1, Tq, Tk], added before scaling.  is_causal: row i
     keeps own key j iff j <= i (top-left, as everywhere in this package; a row that
-    decodes behind a cache needs lengths or a mask instead).
+    decodes behind a cache needs lengths or a mask instead).  Keys that the mask or causality
+    drops get probability 0, which times a value that is not finite is NaN, as in the formula.
     Rows that keep no key at all (no prefix) are NaN, as in the attention.
     Differentiable in query, key, value, prefix_key and prefix_value (the prefix's
     gradients are summed over the batch); ``use_atomic_backward`` as there.
     Returns the output in the input layout.
     """
-    B, Hq, Tq, Tk, D = _dims(query, key, value, layout)
-    Hk = key.shape[1 if layout == "bhsd" else 2]
+    B, Hq, Hk, Tq, Tk, D = _sizes_of(query, key, value, layout)
     _check_prefix(prefix_key, prefix_value, layout, Hk, D)
     _check_types("query", query, key=key, value=value, prefix_key=prefix_key, prefix_value=prefix_value)
     mask, score = _check_sides(mask, score, dict(batch=B, heads=Hq, seqlen_q=Tq, seqlen_k=Tk), query.device)
@@ -380,8 +390,7 @@ def tilelang_attention_with_key_weights(
     Returns (output in the input layout, weights as a new tensor).  For inference: there
     is no gradient, and inputs that ask for one are refused.
     """
-    B, Hq, Tq, Tk, D = _dims(query, key, value, layout)
-    Hk = key.shape[1 if layout == "bhsd" else 2]
+    B, Hq, Hk, Tq, Tk, D = _sizes_of(query, key, value, layout)
     if (prefix_key is None) != (prefix_value is None):
         raise ValueError("prefix_key and prefix_value must be given together")
     if prefix_key is not None:
@@ -448,7 +457,7 @@ def tilelang_evict_keys(
     keeps the last ``recent`` and, of the others, those with the largest ``key_weights``
     (fp32 [B, Hk, Tk]; ties go to the lowest index, NaN counts as the largest), ``keep`` in
     all; with n <= keep all of them.  key, value: [B, Hk, Tk, D] (``layout="bshd"``:
-    [B, Tk, Hk, D]), fp16 / bf16; 1 <= keep <= Tk, 0 <= recent <= keep.
+    [B, Tk, Hk, D]), fp16 / bf16, D up to 256; 1 <= keep <= Tk, 0 <= recent <= keep.
     Returns new tensors: key and value [B, Hk, keep, D] (or bshd) with the kept keys in
     their order, their weights [B, Hk, keep] and their indices in the old cache (int64).
     A sequence holds min(n, keep) keys afterwards; places behind them are zeros, index -1.
@@ -461,8 +470,8 @@ def tilelang_evict_keys(
         raise ValueError("key and value must have the same shape")
     bhsd = layout == "bhsd"
     B, Hk, Tk = key.shape[0], key.shape[1 if bhsd else 2], key.shape[2 if bhsd else 1]
-    if key.shape[3] < 1:
-        raise ValueError("key and value must have a head dimension of at least 1")
+    if not 1 <= key.shape[3] <= 256:
+        raise ValueError(f"head dimension {key.shape[3]} is not supported (1 to 256)")
     _check_types("key", key, value=value)
     keep, recent = int(keep), int(recent)
     if not 1 <= keep <= Tk:
@@ -527,7 +536,8 @@ def tilelang_rotary_embedding(
     (entries of 2^30 and more, infinite ones and NaN turn their pair into NaN).
     sections: how many of the R / 2 pairs turn with each axis, in order (None: one axis).
     Pair i turns by ``positions[axis(i), b, t] * inv_freq[i]``, multiplied in 64-bit fixed
-    point and reduced exactly (off by less than 2^-31 of a turn while |position| < 2^32); it is columns (i, i + R / 2), or (2 i, 2 i + 1) with ``interleaved``:
+    point and reduced exactly (off by less than 2^-31 of a turn while |position| < 2^32); it
+    is columns (i, i + R / 2), or (2 i, 2 i + 1) with ``interleaved``:
     ``(a, b) -> (a cos - b sin, b cos + a sin)``.
     Differentiable in query and key.  Returns new tensors (query, key) in the input layout.
     """
@@ -540,6 +550,8 @@ def tilelang_rotary_embedding(
     B, T, D = query.shape[0], query.shape[t], query.shape[3]
     if key.shape[0] != B or key.shape[t] != T or key.shape[3] != D:
         raise ValueError("query and key must have the same batch size, sequence length and head dimension")
+    if 0 in (query.shape[3 - t], key.shape[3 - t]):
+        raise ValueError("query and key must have at least one head")
     if not 2 <= D <= 256:
         raise ValueError(f"head dimension {D} is not supported (2 to 256)")
     _check_types("query", query, key=key)

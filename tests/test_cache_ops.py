@@ -46,6 +46,9 @@ ATTENTION_REFUSALS = [
     (dict(value=_t(2, 4, 5, 64)), "same number of heads"),
     (dict(value=_t(2, 2, 5, 32)), "same head dimension"),
     (dict(key=_t(2, 3, 5, 64), value=_t(2, 3, 5, 64)), "divisible"),
+    (dict(key=_t(2, 0, 5, 64), value=_t(2, 0, 5, 64)), "at least one head"),
+    (dict(query=_t(2, 8, 3, 0), key=_t(2, 2, 5, 0), value=_t(2, 2, 5, 0)), "one column"),
+    (dict(query=_t(2, 8, 3, 272), key=_t(2, 2, 5, 272), value=_t(2, 2, 5, 272)), "272 is not supported"),
     (dict(query=_t(2, 8, 3, 64, dtype=torch.float32)), "fp16 or bf16"),
     (dict(key=_t(2, 2, 5, 64, dtype=torch.float16)), "same dtype"),
     (dict(prefix_key=_t(2, 7, 64)), "rank-4 tensor of batch size 1"),
@@ -99,6 +102,7 @@ def test_evict_refusals():
         (dict(key=_t(2, 3, 20, 64, dtype=torch.float32)), "fp16 or bf16"),
         (dict(value=_t(2, 3, 20, 64, dtype=torch.float16)), "same dtype"),
         (dict(key=_t(2, 3, 20, 0), value=_t(2, 3, 20, 0)), "head dimension"),
+        (dict(key=_t(2, 3, 20, 264), value=_t(2, 3, 20, 264)), "264 is not supported"),
         (dict(keep=0), "keep"), (dict(keep=21), "keep"), (dict(recent=-1), "recent"), (dict(recent=11), "recent"),
         (dict(key_weights=_t(2, 3, 20)), "key_weights"),
         (dict(key_weights=_t(2, 20, 3, dtype=torch.float32)), "key_weights"),
@@ -118,6 +122,8 @@ def test_rotary_refusals():
         (dict(layout="x"), "unsupported layout"),
         (dict(key=_t(2, 2, 6, 64)), "same batch size"),
         (dict(key=_t(2, 2, 5, 32)), "same batch size"),
+        (dict(query=_t(2, 0, 5, 64)), "at least one head"),
+        (dict(key=_t(2, 0, 5, 64)), "at least one head"),
         (dict(query=_t(2, 8, 5, 258), key=_t(2, 2, 5, 258)), "not supported"),
         (dict(query=_t(2, 8, 5, 64, dtype=torch.float32)), "fp16 or bf16"),
         (dict(key=_t(2, 2, 5, 64, dtype=torch.float16)), "same dtype"),

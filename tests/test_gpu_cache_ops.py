@@ -508,6 +508,18 @@ def test_rotary_far_frequencies(cuda):
     assert torch.equal(y[..., [3, 7]], q[..., [3, 7]])
 
 
+def test_rotary_negative_frequencies(cuda):
+    """Turns backwards, down to frequencies that a double of one turn cannot hold beside it."""
+    g = torch.Generator().manual_seed(33)
+    q = torch.randn((1, 2, 5, 16), generator=g).to(FP)
+    freq = torch.tensor([-1.0, -0.37, -2.0 ** -20, -1e-9, -1e-18, -1e-30, -math.pi, 1e-18])
+    pos = torch.tensor([[[0, 1, -7, 10 ** 9, -2 ** 31]]])
+    angle = OC.angles(pos, freq, (8,))
+    y, _ = api.tilelang_rotary_embedding(q.to(cuda), q.to(cuda), pos.to(cuda), freq.to(cuda))
+    want = OC.turn(q, angle, False)
+    _within("q", y, want, OC.turn_bound(q, want, angle, False, FP))
+
+
 # ---- together, captured, on other streams ------------------------------------------------
 
 
