@@ -42,9 +42,12 @@ MaybeTensor get_opt(const Tensor& x) { return x.defined() ? MaybeTensor(x) : std
 // (multiples of 16), else padded with zeros to their own head dim.
 int64_t columns(int64_t D) { return D % 16 == 0 ? D : kernel_head_dim(D); }
 
+// What memory holds is x (not a view that stands for its negative).
+Tensor as_held(const Tensor& x) { return x.is_neg() ? x.resolve_neg() : x; }
+
 // x as the kernels can address it; copies only where that does not hold.
 Tensor addressable(const Tensor& x, bool bhsd, int64_t W) {
-  Tensor y = x.size(3) == W ? x : at::constant_pad_nd(x, {0, W - x.size(3)});
+  Tensor y = x.size(3) == W ? as_held(x) : at::constant_pad_nd(x, {0, W - x.size(3)});
   return in_place(y, operand(y, bhsd)) ? y : y.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -88,11 +91,18 @@ Tensor side(const Tensor& x, at::ScalarType t, const Tensor& first, int64_t B, i
   TORCH_CHECK(x.dim() == 4 && (x.size(0) == 1 || x.size(0) == B) && (x.size(1) == 1 || x.size(1) == H) && x.size(2) == Tq &&
                   x.size(3) == Tk && x.device() == first.device(),
               "a mask or score must be [batch or 1, heads or 1, rows, keys] on the operands' device");
-  Tensor y = x.scalar_type() == t ? x : x.to(t);
+  Tensor y = as_held(x.scalar_type() == t ? x : x.to(t));
   return y.size(3) == 1 || y.stride(3) == 1 ? y : y.contiguous();
 }
 
-Tensor key_axis_contiguous(const Tensor& x) { return x.size(2) == 1 || x.stride(2) == 1 ? x : x.contiguous(); }
+Tensor key_axis_contiguous(const Tensor& x_) {
+  const Tensor x = as_held(x_);
+  return x.size(2) == 1 || x.stride(2) == 1 ? x : x.contiguous();
+}
+Tensor columns_contiguous(const Tensor& x_) {
+  const Tensor x = as_held(x_);
+  return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous();
+}
 int64_t axis_stride(const Tensor& x, int i) { return x.size(i) == 1 ? 0 : x.stride(i); }
 
 template <typename P> void set_sides(P& p, const Tensor& mask, const Tensor& score, const Tensor& lengths) {
@@ -283,8 +293,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> evict(const Tensor& k_, const Tensor&
   check_lengths(get(lengths_), k_, k_.size(0));
   check_sums(kw_, k_, k_.size(0), k_.size(bhsd ? 1 : 2), k_.size(bhsd ? 2 : 1));
   TORCH_CHECK(keep >= 1 && keep <= k_.size(bhsd ? 2 : 1), "keep must lie in [1, keys]");
-  auto rows = [](const Tensor& x) { return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous(); };
-  const Tensor k = rows(k_), v = rows(v_), kw = key_axis_contiguous(kw_), lengths = get(lengths_);
+  const Tensor k = columns_contiguous(k_), v = columns_contiguous(v_), kw = key_axis_contiguous(kw_), lengths = get(lengths_);
   const Operand ok = operand(k, bhsd), ov = operand(v, bhsd);
   std::vector<int64_t> shape = k.sizes().vec();
   shape[bhsd ? 2 : 1] = keep;
@@ -308,7 +317,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> evict(const Tensor& k_, const Tensor&
 
 using Pair = std::tuple<Tensor, Tensor>;
 
-Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Tensor& freq, const std::vector<int64_t>& sections,
+Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Tensor& freq_, const std::vector<int64_t>& sections,
                 bool adjacent, bool inverse, bool bhsd) {
   check_operands(q_, k_, k_);
   TORCH_CHECK(k_.size(bhsd ? 2 : 1) == q_.size(bhsd ? 2 : 1) && q_.size(bhsd ? 1 : 2) > 0 && k_.size(bhsd ? 1 : 2) > 0,
@@ -317,13 +326,12 @@ Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Ten
                   pos.size(0) == (int64_t)sections.size() && (pos.size(1) == 1 || pos.size(1) == q_.size(0)) &&
                   pos.size(2) == q_.size(bhsd ? 2 : 1),
               "positions must be an int32 or int64 tensor [axes, batch or 1, tokens] on the operands' device");
-  TORCH_CHECK(freq.dim() == 1 && freq.scalar_type() == at::kFloat && freq.is_contiguous() && freq.device() == q_.device() &&
-                  freq.size(0) >= 1 && 2 * freq.size(0) <= q_.size(3),
+  TORCH_CHECK(freq_.dim() == 1 && freq_.scalar_type() == at::kFloat && freq_.is_contiguous() && freq_.device() == q_.device() &&
+                  freq_.size(0) >= 1 && 2 * freq_.size(0) <= q_.size(3),
               "inv_freq must be a contiguous float32 vector on the operands' device");
   const c10::DeviceGuard on_device(q_.device());
   RECORD_FUNCTION("tilelang_fa2_4d_mask::rotary", c10::ArrayRef<const c10::IValue>());
-  auto rows = [](const Tensor& x) { return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous(); };
-  const Tensor q = rows(q_), k = rows(k_);
+  const Tensor q = columns_contiguous(q_), k = columns_contiguous(k_), freq = as_held(freq_);
   const Operand oq = operand(q, bhsd), ok = operand(k, bhsd);
   const Tensor qo = token_major(oq.B, oq.T, oq.H, oq.D, q.options(), bhsd), ko = token_major(ok.B, ok.T, ok.H, ok.D, k.options(), bhsd);
   if (q.numel() == 0) return {qo, ko};

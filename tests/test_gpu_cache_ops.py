@@ -656,6 +656,23 @@ def test_on_another_stream(cuda, name):
                 assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
 
 
+@torch.no_grad()
+def test_negative_views(cuda):
+    """Views that stand for the negative of what memory holds."""
+    (q, k, v, pk, pv, _, w, _, pos, freq), _ = _calls(cuda, 75)
+    neg = lambda x: torch._neg_view(-x)  # noqa: E731
+    s = torch.randn((1, 1, 1, k.shape[2]), generator=torch.Generator().manual_seed(1)).to(cuda)
+    call = api.tilelang_attention_with_key_weights
+    for a, b in ((call(q, k, v, key_weights=w, score=s), call(neg(q), neg(k), neg(v), key_weights=neg(w), score=neg(s))),
+                 ([api.tilelang_shared_prefix_attention(q, k, v, pk, pv)],
+                  [api.tilelang_shared_prefix_attention(q, k, v, neg(pk), neg(pv))]),
+                 (api.tilelang_evict_keys(k, v, w, keep=9), api.tilelang_evict_keys(neg(k), neg(v), neg(w), keep=9)),
+                 (api.tilelang_rotary_embedding(k, v, torch.arange(700, device=cuda).view(1, 1, -1), freq),
+                  api.tilelang_rotary_embedding(neg(k), neg(v), torch.arange(700, device=cuda).view(1, 1, -1), neg(freq)))):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y.resolve_neg())
+
+
 @pytest.mark.parametrize("name", NAMES)
 @torch.no_grad()
 def test_custom_ops_give_the_same(cuda, name):
