@@ -120,13 +120,15 @@ PrefixPlan prefix_plan(const FaPrefixParams* p) {
   const int64_t slots = (p->head_dim > 128 ? 1 : 2) * fa::kCus;
   const int64_t per = std::max<int64_t>(16, ceil_div((f.wide ? 0 : base_p * ntp) + base_o * nto, slots));
   const int64_t per_p = f.wide ? std::max<int64_t>(4, ceil_div(wide_tiles, fa::kCus)) : per;
-  auto ranges = [&](int64_t nt, int64_t per, int* ct) -> int {
-    const int64_t ns = std::min<int64_t>(fa::kPrefixSlots / 2, ceil_div(nt, per));
+  // (half of the join's slots for each key set, and those the other leaves)
+  const int64_t want_p = ceil_div(ntp, per_p), want_o = ceil_div(nto, per);
+  auto ranges = [&](int64_t nt, int64_t want, int64_t other, int* ct) -> int {
+    const int64_t ns = std::min<int64_t>(std::max<int64_t>(fa::kPrefixSlots / 2, fa::kPrefixSlots - other), want);
     *ct = ns ? (int)ceil_div(nt, ns) : 1;
     return ns ? (int)ceil_div(nt, *ct) : 0;
   };
-  f.nsp = ranges(ntp, per_p, &f.ctp);
-  f.nso = ranges(nto, per, &f.cto);
+  f.nsp = ranges(ntp, want_p, want_o, &f.ctp);
+  f.nso = ranges(nto, want_o, want_p, &f.cto);
   f.np = base_p * f.nsp;
   f.no = base_o * f.nso;
   f.nrbp = (int)rbp;

@@ -113,6 +113,10 @@ FORWARD = [
     (17, 32, 8, 128, 2, 4097, 20, FP, None, "rows", None, False, -0.09, "bshd", "contiguous"),
     (23, 48, 16, 96, 1, 4160, 0, BF, None, None, None, False, None, "bhsd", "slice"),
     (65, 16, 16, 80, 1, 4095, 40, BF, "ragged", None, "normal", False, 0.0, "bhsd", "contiguous"),
+    # one key set in more ranges than half of what the join takes; both
+    (1, 4, 1, 64, 1, 0, 40001, BF, "past", None, None, False, None, "bhsd", "contiguous"),
+    (1, 2, 1, 128, 1, 40000, 70, FP, None, None, None, False, None, "bhsd", "contiguous"),
+    (1, 2, 1, 64, 1, 40000, 40000, BF, None, None, None, False, None, "bshd", "contiguous"),
     # more rows per head, on both sides of what decides for the 256-row blocks
     (2, 4, 2, 128, 33, 65, 100, BF, None, None, None, True, None, "bhsd", "token_major"),
     (2, 4, 2, 64, 257, 300, 257, FP, None, None, None, True, None, "bhsd", "contiguous"),
@@ -331,6 +335,7 @@ WEIGHTS = [
     (2, 4, 2, 64, 6, 9, 100, BF, None, "late", "-inf", False, None, "bhsd", "contiguous"),
     (3, 4, 1, 256, 3, 20, 300, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),
     (20, 32, 8, 128, 1, 8200, 77, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),   # (128-row blocks)
+    (1, 4, 2, 64, 1, 0, 45000, BF, None, None, None, False, None, "bhsd", "contiguous"),
     # many rows: the sums in a pass of their own
     (2, 4, 2, 128, 40, 0, 40, BF, None, None, None, True, None, "bhsd", "token_major"),
     (2, 8, 2, 64, 257, 65, 300, FP, "ragged", None, None, False, None, "bshd", "contiguous"),
