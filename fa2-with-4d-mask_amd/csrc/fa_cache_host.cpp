@@ -29,6 +29,7 @@ struct CacheApi {
   const char* (*last_error)();
 };
 CacheApi g_api{};
+PyObject* g_general_backward = nullptr;   // cache.py's prefix backward, held for good
 
 void check(int status, const char* what) {
   TORCH_CHECK(status == FA_OK, what, " failed with status ", status, ": ", g_api.last_error());
@@ -171,6 +172,16 @@ Tensor zeros_past(const Tensor& x, const Tensor& there, bool bhsd) {
   return at::where(bhsd ? there.view({there.size(0), 1, -1, 1}) : there.view({there.size(0), -1, 1, 1}), x, at::zeros({}, x.options()));
 }
 
+// A mask prepared for the kernels that take it so; empty dims are the caller's to exclude.
+Tensor prepared_mask(FaMaskParams m, const at::TensorOptions& bytes) {
+  int64_t n = 0;
+  check(g_api.mask_plan(&m, &n), "fa_mask_plan");
+  const Tensor ws = at::empty({n}, bytes);
+  m.workspace = ws.data_ptr();
+  check(g_api.mask_prepare(&m), "fa_mask_prepare");
+  return ws;
+}
+
 // O (in the caller's layout), LSE [B, Hq, Tq], O's rounding residual and key weights [B, Hk, Tk]
 // (none unless asked for).
 std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& pk_,
@@ -268,12 +279,8 @@ std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> attend(const Tensor& q_, co
     m.batch = p.batch; m.seqlen_q = p.seqlen_q; m.seqlen_k = p.seqlen_k; m.heads_q = p.heads_q;
     m.is_causal = p.is_causal;
     m.stream = p.stream;
-    int64_t n = 0;
-    check(g_api.mask_plan(&m, &n), "fa_mask_plan");
-    mask_ws = at::empty({n}, bytes);
-    m.workspace = mask_ws.data_ptr();
-    check(g_api.mask_prepare(&m), "fa_mask_prepare");
-    p.mask_ws = m.workspace;
+    mask_ws = prepared_mask(m, bytes);
+    p.mask_ws = mask_ws.const_data_ptr();
   }
   const Tensor ws = at::empty({plan.workspace_bytes}, bytes);
   p.workspace = ws.data_ptr();
@@ -281,6 +288,117 @@ std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> attend(const Tensor& q_, co
   check(g_api.prefix_fwd(&p), "fa_prefix_fwd");
   if (kw_too && !p.kw_out) kw_out = key_weights(q, k, lse, get_opt(lengths), get_opt(own_mask), get_opt(score), kw_, scale, causal, bhsd);
   return {first_columns(out, D, bhsd), lse, residual ? MaybeTensor(first_columns(lo, D, bhsd)) : std::nullopt, get_opt(kw_out)};
+}
+
+// dQ, dK, dV, dKp, dVp of a shared prefix as cache.py's prefix_bwd makes them, for operands the
+// kernels take as they lie in memory; false: not for this path.
+bool prefix_backward(const Tensor& dout, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& pk_, const Tensor& pv_,
+                     const Tensor& lengths, const Tensor& mask_, const Tensor& score_, const Tensor& o_, const Tensor& lse,
+                     const Tensor& lo_, double scale, bool causal, bool atomic, bool bhsd, Tensor* out) {
+  for (const Tensor* x : {&q_, &k_, &v_, &pk_, &pv_, &o_, &lse, &lo_})   // (saved tensors come back through hooks)
+    if (!plain(*x) || x->device() != q_.device()) return false;
+  for (const Tensor* x : {&lengths, &mask_, &score_})
+    if (x->defined() && (!plain(*x) || x->device() != q_.device())) return false;
+  if (q_.dim() != 4 || k_.dim() != 4 || pk_.dim() != 4 || q_.size(3) % 16 != 0 || !dout.sizes().equals(q_.sizes()) ||
+      (lengths.defined() && (lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != q_.size(0))))
+    return false;
+  const c10::DeviceGuard on_device(q_.device());
+  auto bthd = [&](const Tensor& x) { return bhsd ? x.transpose(1, 2) : x; };
+  const Tensor d = bthd(dout), q = bthd(q_), k = bthd(k_), v = bthd(v_), pk = bthd(pk_), pv = bthd(pv_), o = bthd(o_), lo = bthd(lo_);
+  const int64_t B = q.size(0), Tq = q.size(1), Hq = q.size(2), D = q.size(3), Tk = k.size(1), Tp = pk.size(1);
+  const int64_t W = kernel_head_dim(D);
+  const bool both = Tp > 0 && Tk > 0;
+  // the sums laid out [Hq, B Tq, W], which is [B, Hq, Tq, W] by strides for the own keys
+  const auto f32 = q.options().dtype(at::kFloat);
+  const Tensor sums = both ? at::empty({Hq, B * Tq, W}, f32) : at::zeros({Hq, B * Tq, W}, f32);
+  Gradients g;
+  if (Tk > 0) {
+    Tensor own_k = k, own_v = v, mask = mask_, mask_ws;
+    if (lengths.defined()) {
+      const Tensor there = existing_keys(lengths, B, Tk);
+      mask = with_lengths(mask, there, B, Tq, Tk);
+      own_k = zeros_past(k, there, false);
+      own_v = zeros_past(v, there, false);
+    }
+    mask = side(mask, at::kBool, q, B, Hq, Tq, Tk);
+    const Tensor score = side(score_, at::kFloat, q, B, Hq, Tq, Tk);
+    if (mask.defined()) {
+      FaMaskParams m{};
+      m.mask = (const uint8_t*)mask.const_data_ptr();
+      m.mask_stride_b = side_stride(mask, 0); m.mask_stride_h = side_stride(mask, 1); m.mask_stride_q = side_stride(mask, 2);
+      m.batch = (int32_t)B; m.seqlen_q = (int32_t)Tq; m.seqlen_k = (int32_t)Tk; m.heads_q = (int32_t)Hq;
+      m.is_causal = causal;
+      m.stream = stream_of(q);
+      mask_ws = prepared_mask(m, q.options().dtype(at::kByte));
+    }
+    const DqSums to{sums, both ? FA_DQ_KEEP : FA_DQ_ADD, Tq * W, B * Tq * W};
+    if (!backward(d, q, own_k, own_v, o, lse, mask, score, mask_ws, lo, scale, causal, atomic, false, &to, &g)) return false;
+    out[0] = bthd(g.dq);
+    out[1] = bthd(g.dk);
+    out[2] = bthd(g.dv);
+  } else {
+    out[1] = at::zeros_like(k_);
+    out[2] = at::zeros_like(v_);
+  }
+  if (Tp > 0) {   // the rows of the batch as one sequence
+    auto one = [&](const Tensor& x) { return x.reshape({1, B * Tq, Hq, D}); };
+    const Tensor lse1 = lse.transpose(0, 1).reshape({1, Hq, B * Tq}).contiguous();
+    const DqSums to{sums, FA_DQ_ADD, 0, B * Tq * W};
+    if (!backward(one(d), one(q), pk, pv, one(o), lse1, Tensor(), Tensor(), Tensor(), one(lo), scale, false, atomic, false, &to, &g))
+      return false;
+    out[0] = bthd(g.dq.view({B, Tq, Hq, D}));
+    out[3] = bthd(g.dk);
+    out[4] = bthd(g.dv);
+  } else {
+    out[3] = at::zeros_like(pk_);
+    out[4] = at::zeros_like(pv_);
+  }
+  return true;
+}
+
+struct Attended {
+  Tensor o, lse, lo, lengths, mask, score;   // the last three as given, undefined where not
+};
+
+struct Prefix : torch::autograd::Function<Prefix> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pk,
+                        const Tensor& pv, const Attended& done, double scale, bool causal, bool atomic, bool bhsd) {
+    ctx->save_for_backward({q, k, v, pk, pv, done.lengths, done.mask, done.score, done.o, done.lse, done.lo});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["flags"] = (int64_t)(causal | atomic << 1 | bhsd << 2);
+    ctx->set_materialize_grads(false);
+    return done.o;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list r(10);
+    if (!grads[0].defined()) return r;   // the output does not reach the loss
+    const auto s = ctx->get_saved_variables();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    const bool causal = flags & 1, atomic = flags >> 1 & 1, bhsd = flags >> 2 & 1;
+    if (plain_backward(grads[0])) {
+      at::AutoDispatchBelowADInplaceOrView below;
+      if (prefix_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10], scale, causal, atomic,
+                          bhsd, r.data()))
+        return r;
+    }
+    pybind11::gil_scoped_acquire gil;
+    const auto g = pybind11::handle(g_general_backward)(grads[0], s[0], s[1], s[2], s[3], s[4], get_opt(s[5]), get_opt(s[6]),
+                                                        get_opt(s[7]), s[8], s[9], s[10], scale, causal, atomic, bhsd)
+                       .cast<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>>();
+    std::tie(r[0], r[1], r[2], r[3], r[4]) = g;
+    return r;
+  }
+};
+
+// O of a shared prefix with its gradients to come.
+Tensor attend_train(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pk, const Tensor& pv, const MaybeTensor& lengths,
+                    const MaybeTensor& mask, const MaybeTensor& score, double scale, bool causal, bool atomic, bool bhsd) {
+  const bool some = pk.size(bhsd ? 2 : 1) > 0;
+  const auto r = attend(q, k, v, some ? MaybeTensor(pk) : std::nullopt, some ? MaybeTensor(pv) : std::nullopt, lengths, mask, score,
+                        std::nullopt, scale, causal, false, true, bhsd);
+  return Prefix::apply(q, k, v, pk, pv, Attended{std::get<0>(r), std::get<1>(r), get(std::get<2>(r)), get(lengths), get(mask), get(score)},
+                       scale, causal, atomic, bhsd);
 }
 
 // K, V and weights of the kept keys, and their indices.
@@ -401,13 +519,14 @@ Pair rotary(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& f
   return rotary_run(q, k, pos, freq, sections, adjacent, inverse, bhsd);
 }
 
-void init_cache(const std::vector<uintptr_t>& fn) {
+void init_cache(const std::vector<uintptr_t>& fn, pybind11::object general) {
   TORCH_CHECK(fn.size() == 9, "nine entry points expected");
   g_api = CacheApi{(decltype(CacheApi::prefix_plan))fn[0],      (decltype(CacheApi::prefix_fwd))fn[1],
                    (decltype(CacheApi::mask_plan))fn[2],        (decltype(CacheApi::mask_prepare))fn[3],
                    (decltype(CacheApi::key_weights_plan))fn[4], (decltype(CacheApi::key_weights))fn[5],
                    (decltype(CacheApi::evict))fn[6],            (decltype(CacheApi::rotary))fn[7],
                    (decltype(CacheApi::last_error))fn[8]};
+  g_general_backward = general.release().ptr();
 }
 
 }  // namespace
@@ -416,6 +535,7 @@ void bind_cache(pybind11::module_& m) {
   using release = pybind11::call_guard<pybind11::gil_scoped_release>;
   m.def("init_cache", &init_cache);
   m.def("attend", &attend, release());
+  m.def("attend_train", &attend_train, release());
   m.def("evict", &evict, release());
   m.def("rotary", &rotary, release());
 }

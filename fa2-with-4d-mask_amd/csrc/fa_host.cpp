@@ -136,13 +136,11 @@ bool forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ma
   return g_api.fwd(&p) == FA_OK;
 }
 
-struct Gradients {
-  Tensor dq, dk, dv;   // in the caller's layout
-};
+}  // namespace
 
-bool backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse,
+bool fa_host::backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse,
               const Tensor& mask, const Tensor& score, const Tensor& mask_ws, const Tensor& o_lo, double scale, bool causal,
-              bool atomic, bool bhsd, Gradients* g) {
+              bool atomic, bool bhsd, const DqSums* sums, Gradients* g) {
   // saved tensors come back through hooks: as the forward saw them, or not here
   const at::ScalarType dt = q.scalar_type();
   auto as_saved = [&](const Tensor& x, at::ScalarType t) { return plain(x) && x.device() == q.device() && x.scalar_type() == t; };
@@ -210,6 +208,10 @@ bool backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor
     p.o_lo = ol.p;
     p.o_lo_stride_b = ol.sb; p.o_lo_stride_t = ol.st; p.o_lo_stride_h = ol.sh;
   }
+  if (sums) {
+    p.dq_mode = sums->mode;
+    p.dq_accum_stride_b = sums->sb; p.dq_accum_stride_h = sums->sh;
+  }
   FaBwdPlan plan{};
   if (g_api.bwd_plan(&p, &plan) != FA_OK) return false;
   RECORD_FUNCTION("tilelang_fa2_4d_mask::bwd", c10::ArrayRef<const c10::IValue>());
@@ -222,7 +224,7 @@ bool backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor
   const Tensor delta = at::empty({2, oq.B, oq.H, oq.T}, f32);   // Delta, backward LSE
   const Tensor dead = at::zeros({oq.B * ok.H}, q.options().dtype(at::kInt));
   Tensor dq_acc, dk_acc, dv_acc, ds;
-  if (plan.needs_dq_accum) dq_acc = at::empty({plan.dq_accum_elems}, f32);
+  if (plan.needs_dq_accum) dq_acc = sums ? sums->sums : at::empty({plan.dq_accum_elems}, f32);
   if (plan.dkv_accum_elems > 0) {
     dk_acc = at::empty({plan.dkv_accum_elems}, f32);
     dv_acc = at::empty({plan.dkv_accum_elems}, f32);
@@ -250,22 +252,10 @@ bool backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor
   return true;
 }
 
-// The Python path's gradients, for what the native one does not take.
-Gradients general_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-                           const Tensor& lse, const Tensor& mask, const Tensor& score, const Tensor& mask_ws,
-                           const Tensor& o_lo, double scale, bool causal, bool atomic, bool bhsd) {
-  pybind11::gil_scoped_acquire gil;
-  auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-  const auto r = pybind11::handle(g_general_backward)(dout, q, k, v, out, lse, opt(mask), opt(score), opt(mask_ws),
-                                                      opt(o_lo), scale, causal, atomic, bhsd)
-                     .cast<std::tuple<Tensor, Tensor, Tensor>>();
-  return {std::get<0>(r), std::get<1>(r), std::get<2>(r)};
-}
-
 // A backward that nothing traces, transforms or intercepts, and no setting that only
 // the Python host path honours (fa2.py _plain_eager, without its Python calls: through
 // them a small step took 6 us longer).
-bool plain_backward(const Tensor& dout) {
+bool fa_host::plain_backward(const Tensor& dout) {
   using K = c10::DispatchKey;
   const auto* meta = torch::autograd::impl::get_autograd_meta(dout);
   if (!plain(dout) || (meta && meta->fw_grad_) || at::GradMode::is_enabled() ||
@@ -277,6 +267,20 @@ bool plain_backward(const Tensor& dout) {
   const pybind11::handle m(g_settings);
   const pybind11::object log = m.attr("_event_log"), limit = m.attr("DS_LIMIT_BYTES");
   return log.is_none() && limit.equal(pybind11::int_(0));
+}
+
+namespace {
+
+// The Python path's gradients, for what the native one does not take.
+Gradients general_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                           const Tensor& lse, const Tensor& mask, const Tensor& score, const Tensor& mask_ws,
+                           const Tensor& o_lo, double scale, bool causal, bool atomic, bool bhsd) {
+  pybind11::gil_scoped_acquire gil;
+  auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+  const auto r = pybind11::handle(g_general_backward)(dout, q, k, v, out, lse, opt(mask), opt(score), opt(mask_ws),
+                                                      opt(o_lo), scale, causal, atomic, bhsd)
+                     .cast<std::tuple<Tensor, Tensor, Tensor>>();
+  return {std::get<0>(r), std::get<1>(r), std::get<2>(r)};
 }
 
 struct Attention : torch::autograd::Function<Attention> {
@@ -303,7 +307,7 @@ struct Attention : torch::autograd::Function<Attention> {
     bool done = false;
     if (plain_backward(grads[0])) {
       at::AutoDispatchBelowADInplaceOrView below;
-      done = ::backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], scale, causal, atomic, bhsd, &g);
+      done = fa_host::backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], scale, causal, atomic, bhsd, nullptr, &g);
     }
     if (!done)
       g = general_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], scale, causal, atomic, bhsd);

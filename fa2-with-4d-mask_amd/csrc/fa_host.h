@@ -52,6 +52,25 @@ inline int dtype_code(const Tensor& q) { return q.scalar_type() == at::kBFloat16
 
 inline void* stream_of(const Tensor& q) { return (void*)c10::hip::getCurrentHIPStream(q.device().index()).stream(); }
 
+// ---- the attention's backward (fa_host.cpp) ----
+
+struct Gradients {
+  Tensor dq, dk, dv;   // in the caller's layout
+};
+// Where dQ is summed in fp32 over several key sets: the sums, FaDqMode, batch and head strides.
+struct DqSums {
+  Tensor sums;
+  int mode;
+  int64_t sb, sh;
+};
+// False: not for the native path.  With `sums` and FA_DQ_KEEP the dQ of `g` is not written.
+bool backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse,
+              const Tensor& mask, const Tensor& score, const Tensor& mask_ws, const Tensor& o_lo, double scale, bool causal,
+              bool atomic, bool bhsd, const DqSums* sums, Gradients* g);
+// A backward that nothing traces, transforms or intercepts, and no setting that only the Python
+// host path honours.
+bool plain_backward(const Tensor& dout);
+
 void bind_cache(pybind11::module_& m);   // fa_cache_host.cpp
 
 }  // namespace fa_host

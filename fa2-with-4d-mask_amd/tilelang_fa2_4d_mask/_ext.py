@@ -256,10 +256,12 @@ def load_host(general_backward=None, settings=None, ds_limit: int = 0):
             raise RuntimeError(f"{HOST_PATH}: ABI version {mod.ABI_VERSION} != {ABI_VERSION}, rebuild it")
         fns = (lib.fa_fwd_plan, lib.fa_fwd, lib.fa_mask_plan, lib.fa_mask_prepare, lib.fa_bwd_plan,
                lib.fa_bwd_preprocess, lib.fa_bwd, lib.fa_bwd_finalize)
-        cache = (lib.fa_prefix_plan, lib.fa_prefix_fwd, lib.fa_mask_plan, lib.fa_mask_prepare, lib.fa_key_weights_plan,
+        entries = (lib.fa_prefix_plan, lib.fa_prefix_fwd, lib.fa_mask_plan, lib.fa_mask_prepare, lib.fa_key_weights_plan,
                  lib.fa_key_weights, lib.fa_evict, lib.fa_rotary, lib.fa_last_error)
         mod.init([ctypes.cast(f, ctypes.c_void_p).value for f in fns], general_backward, settings, ds_limit)
-        mod.init_cache([ctypes.cast(f, ctypes.c_void_p).value for f in cache])
+        from . import cache as _cache
+
+        mod.init_cache([ctypes.cast(f, ctypes.c_void_p).value for f in entries], _cache._general_prefix_backward)
         _host = mod
         return mod
 

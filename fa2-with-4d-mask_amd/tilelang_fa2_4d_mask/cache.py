@@ -284,13 +284,18 @@ def _prefix_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
+def _general_prefix_backward(dO, q, k, v, pk, pv, *rest):
+    """The gradients through the custom op; the native node hands a backward back here that it does
+    not take (a dS limit, the event log, gradients of gradients, operands to copy)."""
+    g = torch.ops.tilelang_fa2_4d_mask.prefix_bwd(dO, q, k, v, pk, pv, *rest)
+    dpk, dpv = (None if x is None else (y if x.numel() else torch.zeros_like(x)) for x, y in ((pk, g[3]), (pv, g[4])))
+    return *g[:3], dpk, dpv
+
+
 def _prefix_backward(ctx, dO, dLSE, dlo):
     if dO is None:
         return (None,) * 13
-    q, k, v, pk, pv, lengths, mask, score, O, LSE, lo = ctx.saved_tensors
-    g = torch.ops.tilelang_fa2_4d_mask.prefix_bwd(dO, q, k, v, pk, pv, lengths, mask, score, O, LSE, lo, *ctx.how)
-    dpk, dpv = (None if x is None else (y if x.numel() else torch.zeros_like(x)) for x, y in ((pk, g[3]), (pv, g[4])))
-    return (*g[:3], dpk, dpv) + (None,) * 8
+    return _general_prefix_backward(dO, *ctx.saved_tensors, *ctx.how) + (None,) * 8
 
 
 prefix_fwd.register_autograd(_prefix_backward, setup_context=_prefix_setup)
@@ -355,9 +360,13 @@ def tilelang_shared_prefix_attention(
     causal, bhsd = bool(is_causal), layout == "bhsd"
     tensors = (query, key, value, prefix_key, prefix_value)
     grad = _wants_grad(*tensors)
-    if not grad and _fa2._plain_eager(*tensors, lengths, mask, score):
-        return _attend(query, key, value, prefix_key, prefix_value, lengths, mask, score, None, scale, causal, False,
-                       False, bhsd)[0]
+    if _fa2._plain_eager(*tensors, lengths, mask, score):
+        if not grad:
+            return _attend(query, key, value, prefix_key, prefix_value, lengths, mask, score, None, scale, causal, False,
+                           False, bhsd)[0]
+        if query.numel() > 0 and key.numel() + prefix_key.numel() > 0:
+            return _host().attend_train(query, key, value, prefix_key, prefix_value, lengths, mask, score, scale, causal,
+                                        bool(use_atomic_backward), bhsd)
     # (the residual of O, for Delta: dQ and dK are sums over many keys and rows in which an error
     # of Delta adds up)
     return torch.ops.tilelang_fa2_4d_mask.prefix_fwd(query, key, value, prefix_key, prefix_value, lengths, mask, score,

@@ -241,6 +241,52 @@ def test_prefix_backward(cuda, case, atomic):
             _within(name, g, w, bound)
 
 
+@pytest.mark.parametrize("case", [
+    ((2, 4, 2, 128, 70, 90, 70), None, None, None, "bhsd"), ((3, 4, 2, 64, 9, 40, 33), "ragged", "rows", "normal", "bshd"),
+    ((2, 4, 2, 96, 33, 0, 40), None, "bernoulli", None, "bhsd"), ((2, 4, 2, 64, 20, 50, 0), None, None, None, "bhsd"),
+    ((2, 4, 2, 40, 12, 20, 30), "ragged", None, None, "bshd"), ((2, 2, 1, 256, 12, 20, 30), "past", None, None, "bhsd")],
+    ids=lambda c: str(c[0]))
+def test_prefix_native_backward(cuda, case):
+    """The native node and the custom ops give the same bits; so do a second backward, saved tensors
+    that went through the host, and a gradient that is laid out otherwise."""
+    from tilelang_fa2_4d_mask.fa2 import record_kernel_events
+
+    shape, lengths, mask, score, layout = case
+    q, k, v, pk, pv, n, m, s = _inputs(11, *shape, BF, lengths, mask, score)
+    if pk is None:
+        pk = pv = q.new_empty((1, shape[2], 0, shape[3]))
+    on = lambda x: None if x is None else x.to(cuda)  # noqa: E731
+    leaves = [_to(x, layout, cuda).requires_grad_(True) for x in (q, k, v, pk, pv)]
+    do = _to(torch.randn(q.shape, generator=torch.Generator().manual_seed(12)).to(BF), layout, cuda)
+
+    def call():
+        return api.tilelang_shared_prefix_attention(*leaves, lengths=on(n), mask=on(m), score=on(s), layout=layout,
+                                                    use_atomic_backward=False)
+
+    def grads(out, do=do, **kw):
+        return torch.autograd.grad(out, leaves, do, **kw)
+
+    out = call()
+    assert "Prefix" in out.grad_fn.name()
+    want = grads(out, retain_graph=True)
+    for x, leaf in zip(want, leaves):
+        assert x.shape == leaf.shape and x.dtype == leaf.dtype
+    other = do.transpose(1, 2).contiguous().transpose(1, 2)
+    with record_kernel_events():
+        op = call()
+        by_op = grads(op)
+    with torch.autograd.graph.save_on_cpu():
+        far = call()
+    for name, got in (("again", grads(out)), ("the ops", by_op), ("saved apart", grads(far)), ("other strides", grads(call(), other))):
+        for x, y in zip(got, want):
+            assert torch.equal(torch.nan_to_num(x), torch.nan_to_num(y)), name
+    out = call()
+    with torch.no_grad():
+        out.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        grads(out)
+
+
 def test_ops_refuse_what_the_wrappers_would(cuda):
     """Called directly, the custom ops check what they are given before they launch."""
     q, k, v, pk, pv, n, m, s = (None if x is None else x.to(cuda) for x in
