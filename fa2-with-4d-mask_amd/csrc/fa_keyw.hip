@@ -5,15 +5,21 @@
 //
 //   key_weights_kernel   a workgroup of 4 waves per (256 keys (128 at head dim 256), part of
 //                        the row tiles, kv-head, sequence).  A wave keeps its 64 (32) keys as MFMA
-//                        operands in registers and walks the rows of the group 32 at a time: S^T
-//                        = K Q^T leaves 16 keys of one row per lane and fragment, which become
-//                        probabilities and are added in place; the sum over the lanes (rows)
-//                        comes once, at the end.  No LDS.  Sums are fp32.
+//                        operands in registers and walks the rows of the group, 64 (32) at a time
+//                        from LDS, where the workgroup's waves share them: S^T = K Q^T leaves 16
+//                        keys of one row per lane and fragment, which become probabilities and are
+//                        added in place; the sum over the lanes (rows) comes once, at the end.
+//                        Sums are fp32.
 //   key_weights_sum_kernel  adds the parts, in order (deterministic), where few key blocks
 //                        leave CUs idle and the row tiles are cut into parts.
 //   far_rows_kernel      with a score: rows whose LSE is so large (masks of the type's lowest
 //                        value in all of the row) that it no longer holds the sum's logarithm get
 //                        their largest raw logit and their sum anew; others leave at once.
+//
+// What bounds it: the exponentials (6 VALU instructions per MFMA at head dim 128, an exp at a quarter
+// of the rate) and the MFMAs, in turn: B1 Tq8192 Tk8192 Hq32/8 D128 causal 399 us, 137 GFLOP at 344
+// TFLOP/s, the MFMA busy a third of the time (each wave with its own loads of the rows: 758 us,
+// the L1s' rate).  More than two waves per SIMD do not fit beside the keys (three: spills, 5 % slower).
 #include "fa_cache.h"
 #include "fa_common.h"
 #include "fa_pipe.h"
@@ -148,28 +154,46 @@ __global__ __launch_bounds__(kWaves * 64, 2) void key_weights_kernel(const KeyWA
       }
       return {g, tq};
     };
-    // A tile's rows and LSEs, loaded while the one before is worked on.
+    // A tile's rows and LSEs, loaded while the one before is worked on.  Rows of one head, as almost
+    // always, lie `off` from its first (with every row's address made on its own the kernel issued 13
+    // VALU instructions per MFMA, now 8.3: B1 Tq8192 Tk8192 Hq32/8 D128 causal 461 -> 399 us).
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
     constexpr int RS = kWaves * 64 / CH;   // rows between a thread's chunks
+    const int col = 8 * c < a.Dv ? 8 * c : 0;
+    int64_t off[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) off[u] = (r0 + u * RS) * a.qst + col;
     u32x4 x[NU];
     float e = 0.f;
     auto load_tile = [&](const Tile& t) __attribute__((always_inline)) {
+      const T* qp = (const T*)a.q + b * a.qsb;
+      const float* lp = a.lse + ((int64_t)b * a.Hq + kvh * a.G) * a.Tq;
+      if (t.tq + RT <= a.Tq) {
+        const T* src = qp + (kvh * a.G + t.g) * a.qsh + (int64_t)t.tq * a.qst;
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const Row q = row_in(t, r0 + u * RS);
-        x[u] = gload16((const T*)a.q + b * a.qsb + (kvh * a.G + q.g) * a.qsh + (int64_t)q.tq * a.qst + (8 * c < a.Dv ? 8 * c : 0));
-      }
-      if (threadIdx.x < RT) {
-        const Row q = row_in(t, threadIdx.x);
-        // rows past R: +inf, as a row without a kept key
-        e = t.t * RT + (int)threadIdx.x < R ? a.lse[((int64_t)b * a.Hq + kvh * a.G + q.g) * a.Tq + q.tq] : kPosInf;
+        for (int u = 0; u < NU; ++u) x[u] = gload16(src + off[u]);
+        if (threadIdx.x < RT) e = lp[(int64_t)t.g * a.Tq + t.tq + threadIdx.x];
+      } else {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const Row q = row_in(t, r0 + u * RS);
+          x[u] = gload16(qp + (kvh * a.G + q.g) * a.qsh + (int64_t)q.tq * a.qst + col);
+        }
+        if (threadIdx.x < RT) {
+          const Row q = row_in(t, threadIdx.x);
+          // rows past R: +inf, as a row without a kept key
+          e = t.t * RT + (int)threadIdx.x < R ? lp[(int64_t)q.g * a.Tq + q.tq] : kPosInf;
+        }
       }
     };
     auto keep_tile = [&](int buf) __attribute__((always_inline)) {
+      if (neg != 0 || a.Dv < D) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) x[u] = zero_unless(8 * c < a.Dv, x[u] ^ neg);
+      }
 #pragma unroll
       for (int u = 0; u < NU; ++u)
-        lds_write16(tiles[buf] + (r0 + u * RS) * 2 * D + ((c ^ swz<D>(r0 + u * RS)) * 16),
-                    zero_unless(8 * c < a.Dv, x[u] ^ neg));
+        lds_write16(tiles[buf] + (r0 + u * RS) * 2 * D + ((c ^ swz<D>(r0 + u * RS)) * 16), x[u]);
       if (threadIdx.x < RT) lses[buf][threadIdx.x] = e;
     };
     // probabilities of 32 rows from LDS (this lane's: row q) added to the keys' sums; EDGE: some are
@@ -244,7 +268,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void key_weights_kernel(const KeyWA
           if (now.t * RT + i >= R || (a.causal && one && now.tq + i + 32 <= k0)) continue;
           const char* rows = tiles[buf] + i * 2 * D;   // (32 rows on: the same swizzle)
           const float lse = lses[buf][i + l32];
-          const Row q = row_in(now, i + l32);
+          const Row q = one ? Row{now.g, now.tq + i + l32} : row_in(now, i + l32);
           if (edge || (a.causal && !(one && now.tq + i >= k0 + 32 * NF - 1))) add(IC<1>{}, rows, q, lse);
           else add(IC<0>{}, rows, q, lse);
         }
