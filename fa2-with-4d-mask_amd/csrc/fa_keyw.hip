@@ -276,24 +276,28 @@ __global__ __launch_bounds__(kWaves * 64, 2) void key_weights_kernel(const KeyWA
       if (t.t < nt) keep_tile(buf ^ 1);   // (its last readers: before the barrier before this one)
       __syncthreads();
     }
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) acc[f][j] += __shfl_xor(acc[f][j], d);
   }
-  // every lane of a half holds the sums of keys 8 (j / 4) + 4 hf + j % 4: lane l32 = j writes one
+  // The sums over a half's 32 lanes, half of the values leaving a lane in every step: lane l32 ends
+  // with that of fragment l32 / 16, value l32 % 16.
+  const bool up = lane & 16;
+  float v[16];
 #pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    float v = acc[f][0];
+  for (int j = 0; j < 16; ++j) {
+    const float mine = NF == 2 && up ? acc[NF - 1][j] : acc[0][j], other = NF == 2 && !up ? acc[NF - 1][j] : acc[0][j];
+    v[j] = mine + __shfl_xor(other, 16);
+  }
 #pragma unroll
-    for (int j = 1; j < 16; ++j) v = l32 == j ? acc[f][j] : v;
-    const int j = k0 + 32 * f + 8 * (l32 >> 2) + 4 * hf + (l32 & 3);
-    if (l32 < 16 && j < a.Tk) {
-      if (a.ns > 1) a.part[((int64_t)sp * a.B * a.Hk + bk) * a.Tk + j] = v;
-      else a.kw_out[(int64_t)bk * a.Tk + j] = v + (a.kw_in ? a.kw_in[b * a.kwsb + kvh * a.kwsh + j] : 0.f);
+  for (int d = 8; d > 0; d >>= 1)
+#pragma unroll
+    for (int j = 0; j < d; ++j) {
+      const bool high = lane & d;
+      const float mine = high ? v[j + d] : v[j], other = high ? v[j] : v[j + d];
+      v[j] = mine + __shfl_xor(other, d);
     }
+  const int j = k0 + (NF == 2 ? 2 * (lane & 16) : 0) + 8 * ((lane & 15) >> 2) + 4 * hf + (lane & 3);
+  if ((NF == 2 || !up) && j < a.Tk) {
+    if (a.ns > 1) a.part[((int64_t)sp * a.B * a.Hk + bk) * a.Tk + j] = v[0];
+    else a.kw_out[(int64_t)bk * a.Tk + j] = v[0] + (a.kw_in ? a.kw_in[b * a.kwsb + kvh * a.kwsh + j] : 0.f);
   }
 }
 
