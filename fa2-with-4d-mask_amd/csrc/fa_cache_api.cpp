@@ -24,6 +24,9 @@ constexpr int64_t kMaxGrid = 1LL << 23;                   // workgroups of 256 t
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// (of positive sizes below 2^31)
+bool rows_fit(int64_t a, int64_t b, int64_t c) { return a * b < kMaxRows && a * b * c < kMaxRows; }
+
 struct Sizes {
   int32_t B, Tq, Tk, Hq, Hk, D, Din, dtype;
   float scale;
@@ -39,7 +42,7 @@ int check_sizes(const Sizes& z, int min_k) {
     return fail(FA_ERR_HEAD_DIM, "head_dim_in %d must be a multiple of 16 up to head_dim %d (0: head_dim)", z.Din, z.D);
   if (z.dtype != FA_DTYPE_BF16 && z.dtype != FA_DTYPE_FP16) return fail(FA_ERR_DTYPE, "unsupported dtype code %d", z.dtype);
   if (!std::isfinite(z.scale)) return fail(FA_ERR_SCALE, "scale must be finite");
-  if ((int64_t)z.B * z.Hq * z.Tq >= kMaxRows || (int64_t)z.B * z.Hk * z.Tk >= kMaxRows)
+  if (!rows_fit(z.B, z.Hq, z.Tq) || !rows_fit(z.B, z.Hk, z.Tk))
     return fail(FA_ERR_SHAPE, "problem too large for 32-bit row indices (B*H*T must stay below 2^31 - 2^16)");
   return FA_OK;
 }
@@ -378,7 +381,7 @@ int fa_evict(const FaEvictParams* p) {
   if (!p) return fail(FA_ERR_NULL, "params is NULL");
   if (p->batch < 1 || p->seqlen_k < 1 || p->heads_k < 1 || p->head_dim < 1)
     return fail(FA_ERR_SHAPE, "sizes must be >= 1 (B=%d Tk=%d Hk=%d D=%d)", p->batch, p->seqlen_k, p->heads_k, p->head_dim);
-  if (p->head_dim > 65536 || (int64_t)p->batch * p->heads_k * p->seqlen_k >= kMaxRows || (int64_t)p->batch * p->heads_k >= (1 << 21))
+  if (p->head_dim > 65536 || (int64_t)p->batch * p->heads_k >= (1 << 21) || !rows_fit(p->batch, p->heads_k, p->seqlen_k))
     return fail(FA_ERR_SHAPE, "problem too large (B*H*T below 2^31 - 2^16, B*H below 2^21)");
   if (p->keep < 1 || p->keep > p->seqlen_k) return fail(FA_ERR_SHAPE, "keep %d must lie in [1, %d]", p->keep, p->seqlen_k);
   if (p->recent < 0 || p->recent > p->keep) return fail(FA_ERR_SHAPE, "recent %d must lie in [0, keep = %d]", p->recent, p->keep);

@@ -381,3 +381,15 @@ def test_dq_modes_of_the_backward(lib):
     one = plan.ds_elems
     assert lib.fa_bwd_plan(ctypes.byref(test_abi.bwd_params(seqlen_q=1024, seqlen_k=1024, dq_mode=1)), ctypes.byref(plan)) == 0
     assert plan.ds_elems == 2 * one
+
+
+def test_sizes_whose_products_overflow(lib):
+    """2^31 - 1 of everything is refused, not multiplied."""
+    most = 2 ** 31 - 1
+    plan, n = _ext.FaPrefixPlan(), ctypes.c_int64()
+    big = dict(batch=most, heads_q=most, heads_k=most, seqlen_k=most)
+    p = prefix_params(seqlen_q=most, seqlen_p=most, **big)
+    assert lib.fa_prefix_plan(ctypes.byref(p), ctypes.byref(plan)) == 2
+    assert lib.fa_key_weights_plan(ctypes.byref(key_weights_params(seqlen_q=most, **big)), ctypes.byref(n)) == 2
+    assert lib.fa_evict(ctypes.byref(evict_params(batch=most, heads_k=most, seqlen_k=most, keep=most))) == 2
+    assert lib.fa_rotary(ctypes.byref(rotary_params(batch=most, seqlen=most, heads_q=most, heads_k=most))) == 2
