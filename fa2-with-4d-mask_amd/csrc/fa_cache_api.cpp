@@ -193,7 +193,7 @@ int prefix_many(const FaPrefixParams* p, const PrefixPlan& f) {
     x.vsb = p->v_stride_b; x.vst = p->v_stride_t; x.vsh = p->v_stride_h;
     x.msb = p->mask_stride_b; x.msh = p->mask_stride_h; x.msq = p->mask_stride_q;
     x.ssb = p->score_stride_b; x.ssh = p->score_stride_h; x.ssq = p->score_stride_q;
-    x.Tk = p->seqlen_k;
+    x.Tk = p->seqlen_k; x.lengths = p->lengths;
     x.causal = causal;
     if (p->mask) {
       x.mws = (const char*)p->mask_ws;
@@ -248,7 +248,8 @@ int fa_prefix_fwd(const FaPrefixParams* p) {
   if (p->kw_out && !(f.few && kw_fits(p)))
     return fail(FA_ERR_SHAPE, "more query rows than key weights are taken with (fa_prefix_plan: few_rows 0)");
   if (!f.few) {
-    if (p->lengths && own) return fail(FA_ERR_SHAPE, "lengths are taken with few rows only (fa_prefix_plan: few_rows 0)");
+    if (p->lengths && own && (p->mask || p->score))
+      return fail(FA_ERR_SHAPE, "lengths beside a mask or score are taken with few rows only (fa_prefix_plan: few_rows 0)");
     if (own && p->mask && !p->mask_ws)
       return fail(FA_ERR_WORKSPACE, "a mask needs its prepared workspace (fa_mask_prepare): mask_ws is NULL");
     if (own && p->mask && (uintptr_t)p->mask_ws % 256) return fail(FA_ERR_STRIDE, "mask_ws must be 256-byte aligned");

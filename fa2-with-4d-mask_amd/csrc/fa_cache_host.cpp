@@ -160,7 +160,7 @@ Tensor key_weights(const Tensor& q_, const Tensor& k_, const Tensor& lse_, const
   return out;
 }
 
-// For kernels that take no lengths and read whole tiles: the own keys' mask with `lengths` as
+// For kernels that take no lengths (a mask's or score's, the backward's) and read whole tiles: the own keys' mask with `lengths` as
 // part of it (rows broadcast), and K or V with zeros past them (0 times what stands there
 // would be NaN if that is no number).
 Tensor existing_keys(const Tensor& lengths, int64_t B, int64_t Tk) { return at::arange(Tk, lengths.options()).lt(lengths.view({B, 1})); }
@@ -228,7 +228,7 @@ std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> attend(const Tensor& q_, co
     check(g_api.prefix_plan(&p, &plan), "fa_prefix_plan");
   }
   Tensor k_clean = k_, v_clean = v_;
-  if (!plan.few_rows && lengths.defined()) {
+  if (!plan.few_rows && lengths.defined() && (mask.defined() || score.defined())) {
     const Tensor there = existing_keys(lengths, B, Tk);
     mask = with_lengths(mask, there, B, Tq, Tk);
     k_clean = zeros_past(k_, there, bhsd);

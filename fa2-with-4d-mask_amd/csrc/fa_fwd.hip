@@ -189,12 +189,13 @@ __global__ __launch_bounds__(fwd_waves(D, CAUSAL, MASK || FINE, SCORE) * 64, fwd
   // range sp of a.ns, of nearly equal counts.  Without a mask a range is taken
   // as a problem of its own whose key 0 is koff (so Tk, tile and key indices
   // below count from koff); with a mask the range is one of list positions.
-  const int kv_end = CAUSAL ? min(a.Tk, q0 + BM) : a.Tk;
+  const int Tk_b = FINE && a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+  const int kv_end = CAUSAL ? min(Tk_b, q0 + BM) : Tk_b;
   const int nt_all = (kv_end + BN - 1) / BN;
   const int t_lo = SPLIT && !MASK ? (int)((int64_t)nt_all * sp / a.ns) : 0;
   const int t_hi = SPLIT && !MASK ? (int)((int64_t)nt_all * (sp + 1) / a.ns) : nt_all;
   const int koff = t_lo * BN;
-  const int Tk = SPLIT && !MASK ? min(a.Tk, t_hi * BN) - koff : a.Tk;
+  const int Tk = SPLIT && !MASK ? min(Tk_b, t_hi * BN) - koff : Tk_b;
 
   const T* __restrict__ qp = (const T*)a.q + b * a.qsb + h * a.qsh;
   const T* __restrict__ kp = (const T*)a.k + b * a.ksb + kvh * a.ksh + (int64_t)koff * a.kst;

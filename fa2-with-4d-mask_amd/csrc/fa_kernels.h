@@ -119,7 +119,8 @@ struct FwdArgs {
   int ns;
   float* part_o;
   float* part_ml;
-  int fine;             // partial results without a mask or score: P in two parts all the same
+  int fine;             // without a mask or score: P in two parts all the same
+  const int32_t* lengths;   // (fine) optional [B]: keys of the sequence that exist, clamped to [0, Tk]
 };
 
 struct PreArgs {

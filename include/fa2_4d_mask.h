@@ -311,7 +311,7 @@ typedef struct FaPrefixParams {
   int32_t is_causal;             /* keep own key j for row i iff j <= i */
   int32_t dtype;
   void* stream;
-  void* workspace;               /* fa_prefix_plan bytes, 16-byte aligned, uninitialised */
+  void* workspace;               /* fa_prefix_plan bytes, 16-byte aligned, uninitialised; NULL for 0 bytes */
   int64_t workspace_bytes;
   const void* mask_ws;           /* the prepared mask (fa_mask_prepare of this mask); required with a mask when
                                     plan.needs_mask_ws */
@@ -320,7 +320,8 @@ typedef struct FaPrefixParams {
 typedef struct FaPrefixPlan {
   int32_t few_rows;              /* 1: rows packed in blocks, the prefix read once for the batch; kw_out and
                                     lengths are taken.  0: the 256-row blocks of fa_fwd for both key sets;
-                                    neither is (lengths as part of the mask, fa_key_weights for the weights) */
+                                    no kw_out (fa_key_weights), lengths only without a mask and score (else
+                                    as part of the mask) */
   int32_t prefix_split;          /* key ranges of the prefix */
   int32_t own_split;             /* key ranges of the own keys */
   int32_t needs_mask_ws;         /* 1: a mask needs its prepared workspace (mask_ws) */

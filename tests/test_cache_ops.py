@@ -247,7 +247,7 @@ PREFIX_REFUSALS = [
     (dict(mask=FAKE, mask_stride_q=-1), 5), (dict(score=FAKE, score_stride_h=-4), 5),
     (dict(kw_in=FAKE, kw_out=FAKE, kw_stride_b=-1), 5), (dict(o_lo=FAKE, o_lo_stride_t=4), 5),
     (dict(workspace=None), 8), (dict(workspace_bytes=100), 8), (dict(workspace=FAKE + 8), 5),
-    (dict(seqlen_q=129, kw_out=FAKE), 2), (dict(seqlen_q=129, lengths=FAKE), 2),
+    (dict(seqlen_q=129, kw_out=FAKE), 2), (dict(seqlen_q=129, lengths=FAKE, score=FAKE), 2),
     (dict(seqlen_q=20, kw_out=FAKE), 2),                       # 80 rows of a group: the weights in a pass of their own
     (dict(seqlen_q=129, mask=FAKE), 8), (dict(seqlen_q=129, mask=FAKE, mask_ws=FAKE + 16), 5),
     (dict(seqlen_q=129, score=FAKE, score_stride_q=1 << 26), 5),

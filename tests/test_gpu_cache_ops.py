@@ -132,6 +132,12 @@ FORWARD = [
     (2, 4, 2, 128, 129, 513, 200, BF, "ragged", "bernoulli", "normal", False, -0.1, "bshd", "contiguous"),
     (1, 8, 8, 40, 170, 180, 170, BF, None, "rows", None, False, 0.0, "bhsd", "contiguous"),
     (2, 4, 2, 64, 300, 77, 500, FP, "past", "late", None, True, None, "bhsd", "contiguous"),
+    # lengths: ranges of one sequence that the next one does not have, none at all
+    (5, 4, 2, 128, 260, 0, 700, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),
+    (5, 4, 2, 64, 200, 300, 900, FP, "ragged", None, None, True, None, "bshd", "token_major"),
+    (3, 2, 2, 96, 150, 0, 2000, BF, "ragged", None, None, False, -0.1, "bhsd", "slice"),
+    (20, 16, 4, 128, 257, 0, 300, BF, "ragged", None, None, True, None, "bhsd", "contiguous"),
+    (20, 16, 4, 64, 270, 30, 300, BF, "past", None, None, False, 0.0, "bhsd", "contiguous"),
     # one range of one key set
     (2, 4, 2, 64, 70, 0, 200, BF, "ragged", "bernoulli", None, True, None, "bhsd", "contiguous"),
     (2, 4, 2, 128, 140, 0, 90, FP, None, None, "normal", False, None, "bshd", "slice"),
@@ -395,6 +401,7 @@ WEIGHTS = [
     (2, 4, 2, 64, 140, 30, 200, FP, None, "late", "lowest", True, None, "bhsd", "contiguous"),
     (2, 8, 2, 128, 131, 300, 299, BF, "ragged", None, None, True, None, "bshd", "contiguous"),
     (1, 6, 2, 128, 700, 0, 520, BF, None, None, None, True, None, "bhsd", "token_major"),
+    (5, 4, 2, 128, 140, 0, 600, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),
 ]
 
 
