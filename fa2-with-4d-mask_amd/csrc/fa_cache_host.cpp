@@ -6,7 +6,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 
-#include <cstring>
+#include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -63,36 +64,92 @@ Tensor first_columns(const Tensor& x, int64_t D, bool bhsd) {
   return bhsd ? x.narrow(3, 0, D).transpose(1, 2).contiguous().transpose(1, 2) : x.narrow(3, 0, D).contiguous();
 }
 
-// What the Python wrappers have checked, again: the custom ops can be called without them.
-void check_like(const Tensor& x, const Tensor& first, const char* name) {
-  TORCH_CHECK(x.dim() == 4 && x.device() == first.device() && x.scalar_type() == first.scalar_type(), name,
-              " must be a rank-4 tensor of the first operand's type and device");
+// What the Python wrappers check, with their texts: nullptr, or why the operands do not fit.  The
+// custom ops can be called without the wrappers, and plain calls come here first (the wrappers' own
+// checks, 4 us a call, then only word the refusal).
+using Why = const char*;
+bool alike(const Tensor& x, const Tensor& first) {
+  return x.dim() == 4 && x.device() == first.device() && x.scalar_type() == first.scalar_type();
 }
-void check_operands(const Tensor& q, const Tensor& k, const Tensor& v) {
-  TORCH_CHECK(q.is_cuda() && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf), "fp16 or bf16 GPU tensors expected");
-  check_like(q, q, "q");
-  check_like(k, q, "k");
-  check_like(v, q, "v");
-  TORCH_CHECK(v.sizes().equals(k.sizes()) && k.size(0) == q.size(0) && k.size(3) == q.size(3) && q.size(3) <= 256,
-              "q, k and v do not fit together, or the head dimension exceeds 256");
+Why operands_misfit(const Tensor& q, const Tensor& k, const Tensor& v) {
+  if (!q.is_cuda() || (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf)) return "fp16 or bf16 GPU tensors expected";
+  if (!alike(q, q) || !alike(k, q) || !alike(v, q)) return "rank-4 tensors of one type on one device expected";
+  if (!v.sizes().equals(k.sizes()) || k.size(0) != q.size(0) || k.size(3) != q.size(3) || q.size(3) > 256)
+    return "q, k and v do not fit together, or the head dimension exceeds 256";
+  return nullptr;
 }
-void check_lengths(const Tensor& n, const Tensor& first, int64_t B) {
-  TORCH_CHECK(!n.defined() || (n.scalar_type() == at::kInt && n.dim() == 1 && n.size(0) == B && n.is_contiguous() &&
-                               n.device() == first.device()),
-              "lengths must be a contiguous int32 tensor of the batch size on the operands' device");
+Why lengths_misfit(const Tensor& n, const Tensor& first) {
+  if (n.defined() && (n.scalar_type() != at::kInt || n.dim() != 1 || n.size(0) != first.size(0) || !n.is_contiguous() ||
+                      n.device() != first.device()))
+    return "lengths must be a contiguous int32 tensor of the batch size on the operands' device";
+  return nullptr;
 }
-void check_sums(const Tensor& w, const Tensor& first, int64_t B, int64_t H, int64_t T) {
-  TORCH_CHECK(!w.defined() || (w.scalar_type() == at::kFloat && w.sizes().equals({B, H, T}) && w.device() == first.device()),
-              "key weights must be a float32 tensor [batch, key heads, keys] on the operands' device");
+Why sums_misfit(const Tensor& w, const Tensor& k, bool bhsd) {
+  if (w.defined() && (w.scalar_type() != at::kFloat || !w.sizes().equals({k.size(0), k.size(bhsd ? 1 : 2), k.size(bhsd ? 2 : 1)}) ||
+                      w.device() != k.device()))
+    return "key weights must be a float32 tensor [batch, key heads, keys] on the operands' device";
+  return nullptr;
+}
+Why side_misfit(const Tensor& x, at::ScalarType t, const Tensor& q, const Tensor& k, bool bhsd) {
+  if (x.defined() && (x.scalar_type() != t || x.dim() != 4 || (x.size(0) != 1 && x.size(0) != q.size(0)) ||
+                      (x.size(1) != 1 && x.size(1) != q.size(bhsd ? 1 : 2)) || x.size(2) != q.size(bhsd ? 2 : 1) ||
+                      x.size(3) != k.size(bhsd ? 2 : 1) || x.device() != q.device()))
+    return "a bool mask or float32 score must be [batch or 1, heads or 1, rows, keys] on the operands' device";
+  return nullptr;
+}
+Why attend_misfit(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pk, const Tensor& pv, const Tensor& lengths,
+                  const Tensor& mask, const Tensor& score, const Tensor& kw, bool bhsd) {
+  const int t = bhsd ? 2 : 1, h = bhsd ? 1 : 2;
+  if (const Why w = operands_misfit(q, k, v)) return w;
+  if (k.size(h) == 0 || q.size(h) % k.size(h) != 0) return "the query heads must be a multiple of the key heads";
+  if (pk.defined() != pv.defined()) return "pk and pv must be given together";
+  if (pk.defined() && (!alike(pk, q) || !alike(pv, q) || !pv.sizes().equals(pk.sizes()) || pk.size(0) != 1 ||
+                       pk.size(h) != k.size(h) || pk.size(3) != q.size(3)))
+    return "pk and pv do not fit k";
+  if (q.numel() == 0 || k.size(t) + (pk.defined() ? pk.size(t) : 0) == 0) return "no rows, or no keys at all";
+  if (const Why w = lengths_misfit(lengths, q)) return w;
+  if (const Why w = side_misfit(mask, at::kBool, q, k, bhsd)) return w;
+  if (const Why w = side_misfit(score, at::kFloat, q, k, bhsd)) return w;
+  return sums_misfit(kw, k, bhsd);
+}
+Why evict_misfit(const Tensor& k, const Tensor& v, const Tensor& kw, const Tensor& lengths, int64_t keep, int64_t recent, bool bhsd) {
+  if (const Why w = operands_misfit(k, k, v)) return w;
+  if (k.numel() == 0) return "no keys";
+  if (const Why w = lengths_misfit(lengths, k)) return w;
+  if (!kw.defined()) return "no key weights";
+  if (const Why w = sums_misfit(kw, k, bhsd)) return w;
+  if (keep < 1 || keep > k.size(bhsd ? 2 : 1)) return "keep must lie in [1, keys]";
+  return recent < 0 || recent > keep ? "recent must lie in [0, keep]" : nullptr;
+}
+Why rotary_misfit(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& freq, const std::vector<int64_t>& sections, bool bhsd) {
+  const int t = bhsd ? 2 : 1, h = bhsd ? 1 : 2;
+  if (const Why w = operands_misfit(q, k, k)) return w;
+  if (k.size(t) != q.size(t) || q.size(h) == 0 || k.size(h) == 0 || q.size(3) < 2) return "q and k do not fit together";
+  const int64_t axes = (int64_t)sections.size();
+  if (pos.dim() != 3 || (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt) || pos.device() != q.device() ||
+      pos.size(0) != axes || (pos.size(1) != 1 && pos.size(1) != q.size(0)) || pos.size(2) != q.size(t))
+    return "positions must be an int32 or int64 tensor [axes, batch or 1, tokens] on the operands' device";
+  if (freq.dim() != 1 || freq.scalar_type() != at::kFloat || !freq.is_contiguous() || freq.device() != q.device() ||
+      freq.size(0) < 1 || 2 * freq.size(0) > q.size(3))
+    return "inv_freq must be a contiguous float32 vector on the operands' device";
+  int64_t sum = 0;
+  for (const int64_t x : sections) {
+    if (x < 0 || x > freq.size(0)) return "a section is negative or too large";
+    sum += x;
+  }
+  return axes < 1 || axes > FA_ROTARY_AXES || sum != freq.size(0) ? "the sections must add up to the pairs of inv_freq, on at most 8 axes" : nullptr;
+}
+bool wants_grad(std::initializer_list<Tensor> xs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& x : xs)
+    if (x.defined() && x.requires_grad()) return true;
+  return false;
 }
 
-// A mask or score [B|1, Hq|1, Tq, Tk] of its type with a contiguous key axis.
-Tensor side(const Tensor& x, at::ScalarType t, const Tensor& first, int64_t B, int64_t H, int64_t Tq, int64_t Tk) {
+// A mask or score [B|1, Hq|1, Tq, Tk] with a contiguous key axis.
+Tensor side(const Tensor& x) {
   if (!x.defined()) return x;
-  TORCH_CHECK(x.dim() == 4 && (x.size(0) == 1 || x.size(0) == B) && (x.size(1) == 1 || x.size(1) == H) && x.size(2) == Tq &&
-                  x.size(3) == Tk && x.device() == first.device(),
-              "a mask or score must be [batch or 1, heads or 1, rows, keys] on the operands' device");
-  Tensor y = as_held(x.scalar_type() == t ? x : x.to(t));
+  const Tensor y = as_held(x);
   return y.size(3) == 1 || y.stride(3) == 1 ? y : y.contiguous();
 }
 
@@ -189,7 +246,8 @@ std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> attend(const Tensor& q_, co
                                                   const MaybeTensor& score_, const MaybeTensor& kw_, double scale, bool causal,
                                                   bool weights, bool residual, bool bhsd) {
   at::AutoDispatchBelowADInplaceOrView below;
-  check_operands(q_, k_, v_);
+  const Why why = attend_misfit(q_, k_, v_, get(pk_), get(pv_), get(lengths_), get(mask_), get(score_), get(kw_), bhsd);
+  TORCH_CHECK(!why, why);
   const c10::DeviceGuard on_device(q_.device());
   RECORD_FUNCTION("tilelang_fa2_4d_mask::prefix_fwd", c10::ArrayRef<const c10::IValue>());
   const int t = bhsd ? 2 : 1, h = bhsd ? 1 : 2;
@@ -204,18 +262,9 @@ std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> attend(const Tensor& q_, co
   p.is_causal = causal;
   p.dtype = dtype_code(q_);
   p.stream = stream_of(q_);
-  if (Tp > 0) {
-    check_like(*pk_, q_, "pk");
-    TORCH_CHECK(pv_, "pk without pv");
-    check_like(*pv_, q_, "pv");
-    TORCH_CHECK(pv_->sizes().equals(pk_->sizes()) && pk_->size(0) == 1 && pk_->size(h) == Hk && pk_->size(3) == D,
-                "pk and pv do not fit k");
-  }
-  check_lengths(get(lengths_), q_, B);
-  check_sums(get(kw_), q_, B, Hk, Tk);
-  const Tensor own_mask = Tk ? side(get(mask_), at::kBool, q_, B, Hq, Tq, Tk) : Tensor();
+  const Tensor own_mask = Tk ? side(get(mask_)) : Tensor();
   Tensor mask = own_mask, lengths = Tk ? get(lengths_) : Tensor();
-  const Tensor score = Tk ? side(get(score_), at::kFloat, q_, B, Hq, Tq, Tk) : Tensor();
+  const Tensor score = Tk ? side(get(score_)) : Tensor();
   set_sides(p, mask, score, lengths);
   const bool kw_too = weights && Tk > 0;
   Tensor kw = get(kw_), kw_out;
@@ -299,8 +348,8 @@ bool prefix_backward(const Tensor& dout, const Tensor& q_, const Tensor& k_, con
     if (!plain(*x) || x->device() != q_.device()) return false;
   for (const Tensor* x : {&lengths, &mask_, &score_})
     if (x->defined() && (!plain(*x) || x->device() != q_.device())) return false;
-  if (q_.dim() != 4 || k_.dim() != 4 || pk_.dim() != 4 || q_.size(3) % 16 != 0 || !dout.sizes().equals(q_.sizes()) ||
-      (lengths.defined() && (lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != q_.size(0))))
+  if (attend_misfit(q_, k_, v_, pk_, pv_, lengths, mask_, score_, Tensor(), bhsd) || q_.size(3) % 16 != 0 ||
+      !dout.sizes().equals(q_.sizes()))
     return false;
   const c10::DeviceGuard on_device(q_.device());
   auto bthd = [&](const Tensor& x) { return bhsd ? x.transpose(1, 2) : x; };
@@ -320,8 +369,8 @@ bool prefix_backward(const Tensor& dout, const Tensor& q_, const Tensor& k_, con
       own_k = zeros_past(k, there, false);
       own_v = zeros_past(v, there, false);
     }
-    mask = side(mask, at::kBool, q, B, Hq, Tq, Tk);
-    const Tensor score = side(score_, at::kFloat, q, B, Hq, Tq, Tk);
+    mask = side(mask);
+    const Tensor score = side(score_);
     if (mask.defined()) {
       FaMaskParams m{};
       m.mask = (const uint8_t*)mask.const_data_ptr();
@@ -405,12 +454,10 @@ Tensor attend_train(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
 std::tuple<Tensor, Tensor, Tensor, Tensor> evict(const Tensor& k_, const Tensor& v_, const Tensor& kw_, const MaybeTensor& lengths_,
                                                  int64_t keep, int64_t recent, bool bhsd) {
   at::AutoDispatchBelowADInplaceOrView below;
+  const Why why = evict_misfit(k_, v_, kw_, get(lengths_), keep, recent, bhsd);
+  TORCH_CHECK(!why, why);
   const c10::DeviceGuard on_device(k_.device());
   RECORD_FUNCTION("tilelang_fa2_4d_mask::evict", c10::ArrayRef<const c10::IValue>());
-  check_operands(k_, k_, v_);
-  check_lengths(get(lengths_), k_, k_.size(0));
-  check_sums(kw_, k_, k_.size(0), k_.size(bhsd ? 1 : 2), k_.size(bhsd ? 2 : 1));
-  TORCH_CHECK(keep >= 1 && keep <= k_.size(bhsd ? 2 : 1), "keep must lie in [1, keys]");
   const Tensor k = columns_contiguous(k_), v = columns_contiguous(v_), kw = key_axis_contiguous(kw_), lengths = get(lengths_);
   const Operand ok = operand(k, bhsd), ov = operand(v, bhsd);
   std::vector<int64_t> shape = k.sizes().vec();
@@ -437,16 +484,8 @@ using Pair = std::tuple<Tensor, Tensor>;
 
 Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Tensor& freq_, const std::vector<int64_t>& sections,
                 bool adjacent, bool inverse, bool bhsd) {
-  check_operands(q_, k_, k_);
-  TORCH_CHECK(k_.size(bhsd ? 2 : 1) == q_.size(bhsd ? 2 : 1) && q_.size(bhsd ? 1 : 2) > 0 && k_.size(bhsd ? 1 : 2) > 0,
-              "q and k do not fit together");
-  TORCH_CHECK(pos.dim() == 3 && (pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) && pos.device() == q_.device() &&
-                  pos.size(0) == (int64_t)sections.size() && (pos.size(1) == 1 || pos.size(1) == q_.size(0)) &&
-                  pos.size(2) == q_.size(bhsd ? 2 : 1),
-              "positions must be an int32 or int64 tensor [axes, batch or 1, tokens] on the operands' device");
-  TORCH_CHECK(freq_.dim() == 1 && freq_.scalar_type() == at::kFloat && freq_.is_contiguous() && freq_.device() == q_.device() &&
-                  freq_.size(0) >= 1 && 2 * freq_.size(0) <= q_.size(3),
-              "inv_freq must be a contiguous float32 vector on the operands' device");
+  const Why why = rotary_misfit(q_, k_, pos, freq_, sections, bhsd);
+  TORCH_CHECK(!why, why);
   const c10::DeviceGuard on_device(q_.device());
   RECORD_FUNCTION("tilelang_fa2_4d_mask::rotary", c10::ArrayRef<const c10::IValue>());
   const Tensor q = columns_contiguous(q_), k = columns_contiguous(k_), freq = as_held(freq_);
@@ -467,7 +506,6 @@ Pair rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos, const Ten
   p.head_dim = (int32_t)oq.D;
   p.rotary = (int32_t)(2 * freq.numel());
   p.axes = (int32_t)sections.size();
-  TORCH_CHECK(sections.size() <= FA_ROTARY_AXES, "at most ", (int)FA_ROTARY_AXES, " axes");
   for (size_t i = 0; i < sections.size(); ++i) p.sections[i] = (int32_t)sections[i];
   p.positions_64 = pos.scalar_type() == at::kLong;
   p.adjacent = adjacent;
@@ -519,6 +557,33 @@ Pair rotary(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& f
   return rotary_run(q, k, pos, freq, sections, adjacent, inverse, bhsd);
 }
 
+// The wrappers' first try: plain calls whose operands fit and need no copies of lengths or score.
+// None: for the wrappers' checks, and the custom ops.
+using MaybeOutputs = std::optional<std::tuple<Tensor, MaybeTensor>>;
+MaybeOutputs attend_plain(const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& v, const MaybeTensor& pk, const MaybeTensor& pv,
+                          const MaybeTensor& lengths, const MaybeTensor& mask, const MaybeTensor& score, const MaybeTensor& kw,
+                          std::optional<double> scale, bool causal, bool weights, bool bhsd) {
+  if (!q || !k || !v || attend_misfit(*q, *k, *v, get(pk), get(pv), get(lengths), get(mask), get(score), get(kw), bhsd) ||
+      wants_grad({*q, *k, *v, get(pk), get(pv), get(score), get(kw)}))
+    return std::nullopt;
+  const bool some = pk && pk->size(bhsd ? 2 : 1) > 0;
+  const double by = scale ? *scale : std::pow((double)q->size(3), -0.5);
+  auto r = attend(*q, *k, *v, some ? pk : std::nullopt, some ? pv : std::nullopt, lengths, mask, score, kw, by, causal, weights, false, bhsd);
+  return std::make_tuple(std::get<0>(r), std::get<3>(r));
+}
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> evict_plain(const MaybeTensor& k, const MaybeTensor& v, const MaybeTensor& kw,
+                                                                      const MaybeTensor& lengths, int64_t keep, int64_t recent, bool bhsd) {
+  if (!k || !v || evict_misfit(*k, *v, get(kw), get(lengths), keep, recent, bhsd) || wants_grad({*k, *v, get(kw)})) return std::nullopt;
+  return evict(*k, *v, *kw, lengths, keep, recent, bhsd);
+}
+std::optional<Pair> rotary_plain(const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& pos, const MaybeTensor& freq,
+                                 std::vector<int64_t> sections, bool adjacent, bool bhsd) {
+  if (!q || !k || !pos || !freq) return std::nullopt;
+  if (sections.empty()) sections = {freq->numel()};
+  if (rotary_misfit(*q, *k, *pos, *freq, sections, bhsd) || wants_grad({*freq})) return std::nullopt;
+  return rotary(*q, *k, *pos, *freq, sections, adjacent, false, bhsd);
+}
+
 void init_cache(const std::vector<uintptr_t>& fn, pybind11::object general) {
   TORCH_CHECK(fn.size() == 9, "nine entry points expected");
   g_api = CacheApi{(decltype(CacheApi::prefix_plan))fn[0],      (decltype(CacheApi::prefix_fwd))fn[1],
@@ -536,8 +601,11 @@ void bind_cache(pybind11::module_& m) {
   m.def("init_cache", &init_cache);
   m.def("attend", &attend, release());
   m.def("attend_train", &attend_train, release());
+  m.def("attend_plain", &attend_plain, release());
   m.def("evict", &evict, release());
+  m.def("evict_plain", &evict_plain, release());
   m.def("rotary", &rotary, release());
+  m.def("rotary_plain", &rotary_plain, release());
 }
 
 }  // namespace fa_host

@@ -119,6 +119,12 @@ def _host():
     return _ext.load_host()
 
 
+def _plain(layout: str, first, *others) -> bool:
+    """A plain eager call on GPU tensors: the native path tries it before any check here (it
+    returns None unless the operands fit, as the checks here would have it)."""
+    return getattr(first, "is_cuda", False) and layout in ("bhsd", "bshd") and _fa2._plain_eager(first, *others)
+
+
 def _timed(entry: str, fn, *args):
     """fn(*args), recorded under the library entry's name where an event log is open
     (fa2.py record_kernel_events)."""
@@ -350,6 +356,11 @@ def tilelang_shared_prefix_attention(
     gradients are summed over the batch); ``use_atomic_backward`` as there.
     Returns the output in the input layout.
     """
+    if _plain(layout, query, key, value, prefix_key, prefix_value, lengths, mask, score) and prefix_key is not None:
+        r = _host().attend_plain(query, key, value, prefix_key, prefix_value, lengths, mask, score, None,
+                                 None if scale is None else float(scale), bool(is_causal), False, layout == "bhsd")
+        if r is not None:
+            return r[0]
     B, Hq, Hk, Tq, Tk, D = _sizes_of(query, key, value, layout)
     _check_prefix(prefix_key, prefix_value, layout, Hk, D)
     _check_types("query", query, key=key, value=value, prefix_key=prefix_key, prefix_value=prefix_value)
@@ -399,6 +410,11 @@ def tilelang_attention_with_key_weights(
     Returns (output in the input layout, weights as a new tensor).  For inference: there
     is no gradient, and inputs that ask for one are refused.
     """
+    if _plain(layout, query, key, value, prefix_key, prefix_value, lengths, mask, score, key_weights):
+        r = _host().attend_plain(query, key, value, prefix_key, prefix_value, lengths, mask, score, key_weights,
+                                 None if scale is None else float(scale), bool(is_causal), True, layout == "bhsd")
+        if r is not None:
+            return r
     B, Hq, Hk, Tq, Tk, D = _sizes_of(query, key, value, layout)
     if (prefix_key is None) != (prefix_value is None):
         raise ValueError("prefix_key and prefix_value must be given together")
@@ -471,6 +487,10 @@ def tilelang_evict_keys(
     their order, their weights [B, Hk, keep] and their indices in the old cache (int64).
     A sequence holds min(n, keep) keys afterwards; places behind them are zeros, index -1.
     """
+    if _plain(layout, key, value, key_weights, lengths):
+        r = _host().evict_plain(key, value, key_weights, lengths, int(keep), int(recent), layout == "bhsd")
+        if r is not None:
+            return r
     if key.dim() != 4 or value.dim() != 4:
         raise ValueError("key and value must be rank-4 tensors")
     if layout not in ("bhsd", "bshd"):
@@ -550,6 +570,11 @@ def tilelang_rotary_embedding(
     ``(a, b) -> (a cos - b sin, b cos + a sin)``.
     Differentiable in query and key.  Returns new tensors (query, key) in the input layout.
     """
+    sections = None if sections is None else [int(x) for x in sections]
+    if sections != [] and _plain(layout, query, key, positions, inv_freq):
+        r = _host().rotary_plain(query, key, positions, inv_freq, sections or [], bool(interleaved), layout == "bhsd")
+        if r is not None:
+            return r
     if query.dim() != 4 or key.dim() != 4:
         raise ValueError("query and key must be rank-4 tensors")
     if layout not in ("bhsd", "bshd"):
@@ -569,7 +594,7 @@ def tilelang_rotary_embedding(
     pairs = inv_freq.shape[0]
     if not 1 <= pairs <= D // 2:
         raise ValueError(f"inv_freq must have 1 to {D // 2} entries, got {pairs}")
-    sections = [pairs] if sections is None else [int(x) for x in sections]
+    sections = [pairs] if sections is None else sections
     if not 1 <= len(sections) <= _ext.ROTARY_AXES or min(sections) < 0 or sum(sections) != pairs:
         raise ValueError(f"sections must be 1 to {_ext.ROTARY_AXES} counts that add up to the {pairs} pairs of inv_freq")
     if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 3:
