@@ -116,12 +116,14 @@ PrefixPlan prefix_plan(const FaPrefixParams* p) {
   const int64_t rbp = ceil_div(TG * p->batch, rows_p), rbo = ceil_div(TG, 32);
   const int64_t ntp = ceil_div(p->seqlen_p, keys_p), nto = ceil_div(p->seqlen_k, kt);
   const int64_t base_p = ntp ? p->heads_k * rbp : 0, base_o = nto ? (int64_t)p->batch * p->heads_k * rbo : 0;
-  // Tiles per range: one round of workgroups (two per CU; wide ones beside the own keys': one),
-  // four tiles for every wave where there are as many, no more slots than the join holds.
-  // (B16 Tp8192: ranges of 4 tiles 26.7 us, 16 16.9, 24 18.0; own keys of B64 Tk512 in two rounds 28.3, in
-  // one 24.8.)
+  // Tiles per range: one round of workgroups (two per CU; wide ones beside the own keys': one), four
+  // tiles for every wave where there are as many, fewer only until every CU has a workgroup; no
+  // more slots than the join holds.  (B16 Tp8192: ranges of 4 tiles 26.7 us, 16 16.9, 24 18.0; own keys of
+  // B64 Tk512 in two rounds 28.3, in one 24.8; B1 Hq32 Hk8 own 1000: ranges of 16 tiles 11.8, of 4 8.6;
+  // B12 Tq7 Hq24 Hk8 Tp1000: 16 15.0, 8 13.7, 4, two workgroups per CU, 17.8.)
   const int64_t slots = (p->head_dim > 128 ? 1 : 2) * fa::kCus;
-  const int64_t per = std::max<int64_t>(16, ceil_div((f.wide ? 0 : base_p * ntp) + base_o * nto, slots));
+  const int64_t work = (f.wide ? 0 : base_p * ntp) + base_o * nto;
+  const int64_t per = std::max(std::min<int64_t>(16, std::max<int64_t>(4, ceil_div(work, fa::kCus))), ceil_div(work, slots));
   const int64_t per_p = f.wide ? std::max<int64_t>(4, ceil_div(wide_tiles, fa::kCus)) : per;
   // (half of the join's slots for each key set, and those the other leaves)
   const int64_t want_p = ceil_div(ntp, per_p), want_o = ceil_div(nto, per);
