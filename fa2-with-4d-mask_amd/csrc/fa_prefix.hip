@@ -28,7 +28,7 @@
 // 43 us with the join (35 + 8 in a profile), 3.2 TB/s: 17 MB of fp32 partial results of the
 // prefix's ranges go out and come back, and the sequences' own ranges are short.  Own keys alone,
 // long enough: B1 Hk8 1e6 keys 667 us, 6.1 TB/s; B16 Tk 4096 with key weights, 208 MB in 55 us.  A few
-// rows (B4 Tp1000): latency, 8 + 5 us of two launches beside 11 us of host time.
+// rows (B4 Tp1000): latency, 6 + 5 us of two launches beside 11 us of host time.
 #include "fa_cache.h"
 #include "fa_common.h"
 
