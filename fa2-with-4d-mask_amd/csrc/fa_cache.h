@@ -34,7 +34,11 @@ struct PrefixArgs {
 };
 constexpr int kPrefixSlots = 128;     // most key ranges of a problem: two per lane of the joining wave
 constexpr int kWideRows = 128;
-constexpr int kPrefixKwRows = 64;     // most rows of a kv-head's group with kw_out
+// Most rows of a kv-head's group with kw_out: each leaves its logits, 4 bytes a key to write and read
+// again; past them a pass of its own over K is shorter.  Together / apart in us (bf16, D 128): B1
+// Tk16000 Hq32 Hk8 4 rows of a group 20 / 30, 16 27.4 / 30.3, 32 38 / 31, 64 65 / 38; B8 Tk8000 16
+// 78 / 94, 32 95 / 97, 64 160 / 118; B1 Tk3000 32 30 / 21.6; B16 Tk<=4096 Hq32 Hk8 4 55 / 85.
+constexpr int kPrefixKwRows = 16;
 int prefix_tile_keys();
 hipError_t launch_prefix_rows(const PrefixArgs& a, int D, int dtype, hipStream_t s);
 hipError_t launch_prefix_join(const PrefixArgs& a, int D, int dtype, hipStream_t s);

@@ -388,7 +388,9 @@ WEIGHTS = [
     (3, 4, 1, 256, 3, 20, 300, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),
     (20, 32, 8, 128, 1, 8200, 77, BF, "ragged", None, None, False, None, "bhsd", "contiguous"),   # (128-row blocks)
     (1, 4, 2, 64, 1, 0, 45000, BF, None, None, None, False, None, "bhsd", "contiguous"),
-    # many rows: the sums in a pass of their own
+    (2, 6, 2, 96, 5, 33, 300, BF, "ragged", "bernoulli", None, True, None, "bhsd", "slice"),
+    (3, 16, 1, 128, 1, 40, 290, FP, "past", "rows", "normal", False, 0.0, "bshd", "contiguous"),
+    # more rows: the sums in a pass of their own
     (2, 4, 2, 128, 40, 0, 40, BF, None, None, None, True, None, "bhsd", "token_major"),
     (2, 8, 2, 64, 257, 65, 300, FP, "ragged", None, None, False, None, "bshd", "contiguous"),
     (1, 16, 2, 96, 300, 0, 300, BF, None, "bernoulli", None, True, None, "bhsd", "contiguous"),
