@@ -18,7 +18,9 @@
 //
 // Measured: B1 Tk 16384 Hk8 D128 keep 4096 16.4 us, 33.7 MB of rows and weights at 2.1 TB/s (head
 // dim 8, the selection almost alone, 13.0; the most recent ones alone, without it, 11.4, of which
-// a launch takes some 5); B16 Tk 3001 Hk4 D96 keep 1500 19.7 us, 74 MB at 3.7 TB/s.
+// a launch takes some 5); B16 Tk 3001 Hk4 D96 keep 1500 19.7 us, 74 MB at 3.7 TB/s; B64 Tk 4096 Hk8 D128
+// keep 2048 224 us, 4.8 TB/s.  Past the LDS every workgroup goes over all weights four times: B1 Tk
+// 131072 Hk8 D128 keep 32768 130 us, about half of it the copies.
 #include "fa_cache.h"
 #include "fa_common.h"
 
@@ -202,8 +204,11 @@ __global__ __launch_bounds__(kThreads) void evict_kernel(const EvictArgs a) {
     seen += i < wave ? hist[kWaves + i] : 0;
   }
   // ---- this workgroup's places [i0, i1), filled by the waves whose keys go there ---------------
+  const int first = (int)(before + min(seen, ties)) - i0;   // the wave's own places [first, end)
+  const int end = (int)(before + __builtin_amdgcn_readlane((int)gt, 63) +
+                        min(seen + __builtin_amdgcn_readlane((int)eq, 63), ties)) - i0;
 #pragma unroll 1
-  for (int c0 = 0; c0 < np; c0 += 64) {
+  for (int c0 = 0; c0 < np && first < share && end > 0; c0 += 64) {
     if constexpr (CAP == 0) bits(c0);   // (else one round: the bits are there)
     const uint32_t ng = __popcll(more), ne = __popcll(same);
     const uint32_t ig = wave_scan(ng), ie = wave_scan(ne), e = seen + ie - ne;
