@@ -393,3 +393,15 @@ def test_sizes_whose_products_overflow(lib):
     assert lib.fa_key_weights_plan(ctypes.byref(key_weights_params(seqlen_q=most, **big)), ctypes.byref(n)) == 2
     assert lib.fa_evict(ctypes.byref(evict_params(batch=most, heads_k=most, seqlen_k=most, keep=most))) == 2
     assert lib.fa_rotary(ctypes.byref(rotary_params(batch=most, seqlen=most, heads_q=most, heads_k=most))) == 2
+
+
+@pytest.mark.parametrize("over,few", [
+    (dict(seqlen_q=128), 1), (dict(seqlen_q=129), 0), (dict(seqlen_q=64, seqlen_p=100), 1), (dict(seqlen_q=65, seqlen_p=100), 0),
+    (dict(seqlen_q=4000, head_dim=256), 1), (dict(seqlen_q=4, kw_out=FAKE), 1), (dict(seqlen_q=5, kw_out=FAKE), 0),
+    (dict(seqlen_q=5, heads_q=8, kw_out=FAKE), 1),
+])
+def test_prefix_plan_rows(lib, over, few):
+    """Which calls run packed, and keep the logits that key weights need."""
+    plan = _ext.FaPrefixPlan()
+    assert lib.fa_prefix_plan(ctypes.byref(prefix_params(**over)), ctypes.byref(plan)) == 0
+    assert plan.few_rows == few and 1 <= plan.prefix_split + plan.own_split <= 128
